@@ -562,6 +562,42 @@ TGT_API int tgt_embedding_sum_grad(const float* dout, const int64_t* ids, int64_
                                    int hidden, int64_t padding_idx, float* dtable, void* scratch, size_t scratch_bytes,
                                    void* stream);
 
+/*
+ * Root-mean-square norm of rows, with the residual addition in front of it: v = x + residual (NULL: v = x), y = v rstd weight
+ * with rstd = 1 / sqrt(mean(v^2) + eps), in fp32 from tensors of `dtype` (TGT_F32 or TGT_BF16, all of the same); sum (may be
+ * NULL) receives v, rstd (may be NULL) one fp32 value a row.  hidden is 1 to 16384 (TGT_ERR_UNSUPPORTED above).  Rows of
+ * whole 16-byte pieces from 16-byte boundaries on move in such pieces, others value by value.
+ *   e4m3:     the same with y in 8 bits: scales [rows] = max(max |y| / 448, 2^-126) and values [rows, hidden] = y / scale, to
+ *             the nearest e4m3 number.  A row with a NaN or an infinity has a NaN scale.
+ *   backward: dx = rstd (dy weight - u mean(dy weight u)) + dsum with u = v rstd, dsum (may be NULL) the gradient of sum, v
+ *             what the forward had as x or stored as sum; dweight [hidden] = sum over rows of dy u, fixed order.
+ */
+TGT_API int tgt_rms_norm_fwd(const void* x, const void* residual, const void* weight, float eps, int64_t rows, int hidden,
+                             int dtype, void* sum, void* y, float* rstd, void* stream);
+TGT_API int tgt_rms_norm_e4m3(const void* x, const void* residual, const void* weight, float eps, int64_t rows, int hidden,
+                              int dtype, void* sum, void* values, float* scales, void* stream);
+TGT_API int tgt_rms_norm_bwd_scratch_bytes(int64_t rows, int hidden, int dtype, size_t* bytes);
+TGT_API int tgt_rms_norm_bwd(const void* dy, const void* dsum, const void* v, const void* weight, const float* rstd,
+                             int64_t rows, int hidden, int dtype, void* dx, void* dweight, void* scratch,
+                             size_t scratch_bytes, void* stream);
+
+/*
+ * Learned relative position bias of edges: bias [n_edges, heads] = table[bucket] for edge_index [2, n_edges] (sources, then
+ * destinations; int64 where wide_ids, else int32), positions [n_positions] of the nodes (int64 where wide_positions; NULL: a
+ * node's position is its id), and table [n_buckets, heads] fp32.  borders is a HOST array of n_borders positive numbers in
+ * order: a distance's bucket is the number of borders up to it.  both_ways: n_buckets = 2 (n_borders + 1), the second half for
+ * sources behind their destination (position[source] > position[destination]); else n_buckets = n_borders + 1 and those have
+ * distance 0.  At most 512 buckets and 256 heads (TGT_ERR_UNSUPPORTED).  buckets (may be NULL) receives the buckets, 0xffff
+ * for an edge with an id outside the positions, whose bias is NaN and which has no part in the gradient.
+ * The gradient: dtable [n_buckets, heads] = sum of the rows of dbias in every bucket, fixed order.
+ */
+TGT_API int tgt_edge_position_bias(const void* edge_index, int64_t n_edges, int wide_ids, const void* positions,
+                                   int64_t n_positions, int wide_positions, const int32_t* borders, int n_borders,
+                                   int both_ways, const float* table, int heads, float* bias, uint16_t* buckets, void* stream);
+TGT_API int tgt_edge_position_bias_grad_scratch_bytes(int64_t n_edges, int n_buckets, int heads, size_t* bytes);
+TGT_API int tgt_edge_position_bias_grad(const float* dbias, const uint16_t* buckets, int64_t n_edges, int n_buckets, int heads,
+                                        float* dtable, void* scratch, size_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -493,4 +493,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("attention_backward", &backward_pass, Unlocked());
   bind_batching(m);
   bind_dense(m);
+  bind_block(m);
 }

@@ -127,5 +127,6 @@ at::Tensor attention_over_rows(const at::Tensor& q, const at::Tensor& k, const a
 
 void bind_batching(pybind11::module_& m);   // binding_batch.cpp
 void bind_dense(pybind11::module_& m);      // binding_dense.cpp
+void bind_block(pybind11::module_& m);      // binding_block.cpp
 
 }  // namespace tgt_host

@@ -1,0 +1,225 @@
+// Autograd nodes of the operators around the attention of a pre-norm block: the root-mean-square norm
+// (torchgt_b200/rms_norm.py), the learned relative position bias (torchgt_b200/position_bias.py) and the gated feed-forward
+// block (torchgt_b200/gated_ffn.py).
+#include "binding.h"
+
+#include <ATen/TensorSubclassLikeUtils.h>
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <pybind11/stl.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/utils/pybind.h>
+
+namespace tgt_host {
+namespace {
+
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+// a CUDA tensor of the kernels' types, not a functorch wrapper, a dual number, a fake or a lazily negated view
+bool plain(const at::Tensor& t, const at::Device& device, at::ScalarType type) {
+  return t.defined() && !at::isTensorSubclassLike(t) && t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == type &&
+         t.device() == device && !torch::autograd::isFwGradDefined(t) && !t.is_neg();
+}
+bool kernel_type(at::ScalarType type) { return type == at::kFloat || type == at::kBFloat16; }
+int type_code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? TGT_F32 : TGT_BF16; }
+
+at::Tensor scratch_of(size_t bytes, const at::Tensor& like) {
+  return at::empty({int64_t(bytes < 16 ? 16 : bytes)}, like.options().dtype(at::kByte));
+}
+
+// ---- root-mean-square norm, with the residual addition in front of it -----------------------------------------------
+// Outputs: the normalised rows and, with a residual, x + residual.
+struct RmsNormRowsBackward : public torch::autograd::Node {
+  SavedVariable normalised, weight, rstd;   // the norm's input: x, or the output x + residual
+  bool with_residual = false;
+  double eps = 0;
+
+  // With create_graph the gradient is itself differentiated, with is_grads_batched there are many: the formula as operations.
+  variable_list recorded(const at::Tensor& dy_, const at::Tensor& ds, const at::Tensor& v_, const at::Tensor& w_) {
+    const at::Tensor v = v_.to(at::kFloat), w = w_.to(at::kFloat);
+    const at::Tensor r = (v * v).mean(-1, true).add(eps).rsqrt(), u = v * r;
+    at::Tensor dx, dw;
+    if (dy_.defined()) {
+      const at::Tensor dy = dy_.to(at::kFloat), g = dy * w;
+      dx = r * (g - u * (g * u).mean(-1, true));
+      dw = (dy * u).reshape({-1, w.numel()}).sum(0).to(w_.scalar_type());
+    }
+    if (ds.defined()) dx = dx.defined() ? dx + ds.to(at::kFloat) : ds;
+    dx = dx.to(v_.scalar_type());
+    return {dx, with_residual ? dx : at::Tensor(), dw};
+  }
+
+  variable_list apply(variable_list&& grads) override {
+    return reporting([&] { return backward(grads); });
+  }
+  variable_list backward(const variable_list& grads) {
+    const at::Tensor ds = with_residual ? grads[1] : at::Tensor();
+    if (!grads[0].defined()) return {ds, ds, at::Tensor()};              // only x + residual was used, or nothing
+    const at::Tensor v = with_residual ? normalised.unpack(shared_from_this()) : normalised.unpack();
+    const at::Tensor w = weight.unpack(), rstd_ = rstd.unpack();
+    if (at::GradMode::is_enabled() || at::isTensorSubclassLike(grads[0]) || (ds.defined() && at::isTensorSubclassLike(ds)))
+      return recorded(grads[0], ds, v, w);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(v.device());
+    const at::Tensor dy = grads[0].contiguous(), vc = v.contiguous(), wc = w.contiguous();
+    const at::Tensor dsum = ds.defined() ? ds.contiguous() : ds;
+    const int64_t hidden = w.numel(), rows = v.numel() / hidden;
+    const at::Tensor dx = at::empty(v.sizes(), dy.options()), dw = at::empty(w.sizes(), dy.options());
+    size_t bytes = 0;
+    check(tgt_rms_norm_bwd_scratch_bytes(rows, int(hidden), type_code(v), &bytes));
+    const at::Tensor scratch = scratch_of(bytes, dy);
+    check(tgt_rms_norm_bwd(ptr(dy), ptr(dsum), ptr(vc), ptr(wc), fptr(rstd_), rows, int(hidden), type_code(v), ptr(dx), ptr(dw),
+                           scratch.data_ptr(), scratch.numel(), stream_of(dy)));
+    return {dx, with_residual ? dx : at::Tensor(), dw};
+  }
+  std::string name() const override { return "RmsNormRowsBackward"; }
+  void release_variables() override {
+    normalised.reset_data();
+    weight.reset_data();
+    rstd.reset_data();
+  }
+};
+
+bool rms_norm_covers(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& residual) {
+  constexpr int64_t kMostHidden = 16384;
+  if (!x.defined() || at::isTensorSubclassLike(x) || !kernel_type(x.scalar_type())) return false;
+  if (!plain(x, x.device(), x.scalar_type()) || !plain(w, x.device(), x.scalar_type())) return false;
+  if (w.dim() != 1 || x.dim() < 1 || x.size(-1) != w.numel() || w.numel() < 1 || w.numel() > kMostHidden) return false;
+  return !residual.has_value() || (plain(*residual, x.device(), x.scalar_type()) && residual->sizes() == x.sizes());
+}
+
+// {norm of x (+ residual), x + residual or nothing}; the sum is left out when nobody wants it
+std::pair<at::Tensor, std::optional<at::Tensor>> add_rms_norm(const at::Tensor& x, const std::optional<at::Tensor>& residual_in,
+                                                              const at::Tensor& w, double eps, bool want_sum) {
+  TORCH_CHECK(rms_norm_covers(x, w, residual_in), "rms_norm: tensors that the kernels do not cover");
+  const at::Tensor residual = residual_in.value_or(at::Tensor());
+  const c10::cuda::CUDAGuard guard(x.device());
+  const bool record = torch::autograd::compute_requires_grad(x, residual, w);
+  const int64_t hidden = w.numel(), rows = x.numel() / hidden;
+  at::Tensor y, sum, rstd;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor xc = x.contiguous(), wc = w.contiguous(), rc = residual.defined() ? residual.contiguous() : residual;
+    y = at::empty(x.sizes(), x.options());
+    if (residual.defined() && (want_sum || record)) sum = at::empty(x.sizes(), x.options());
+    if (record) rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+    check(tgt_rms_norm_fwd(ptr(xc), ptr(rc), ptr(wc), float(eps), rows, int(hidden), type_code(x), ptr(sum), ptr(y),
+                           record ? fptr(rstd) : nullptr, stream_of(x)));
+  }
+  if (record) {
+    auto node = std::shared_ptr<RmsNormRowsBackward>(new RmsNormRowsBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, residual, w));
+    node->with_residual = residual.defined();
+    node->eps = eps;
+    node->rstd = SavedVariable(rstd, false);
+    node->weight = SavedVariable(w, false);
+    if (residual.defined()) {
+      torch::autograd::set_history(variable_list{y, sum}, node);
+      node->normalised = SavedVariable(sum, true);
+    } else {
+      torch::autograd::set_history(y, node);
+      node->normalised = SavedVariable(x, false);
+    }
+  }
+  return {y, sum.defined() ? std::optional<at::Tensor>(sum) : std::nullopt};
+}
+
+// {values, scales, x + residual or nothing}; no gradients
+std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>> rms_norm_e4m3(const at::Tensor& x, const at::Tensor& w, double eps,
+                                                                            const std::optional<at::Tensor>& residual_in) {
+  TORCH_CHECK(rms_norm_covers(x, w, residual_in), "rms_norm_quantized: tensors that the kernels do not cover");
+  const at::AutoDispatchBelowADInplaceOrView below;
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t hidden = w.numel(), rows = x.numel() / hidden;
+  const at::Tensor xc = x.contiguous(), wc = w.contiguous();
+  at::Tensor rc, sum;
+  if (residual_in.has_value()) {
+    rc = residual_in->contiguous();
+    sum = at::empty(x.sizes(), x.options());
+  }
+  const at::Tensor values = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  const at::Tensor scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  check(tgt_rms_norm_e4m3(ptr(xc), ptr(rc), ptr(wc), float(eps), rows, int(hidden), type_code(x), ptr(sum), ptr(values),
+                          fptr(scales), stream_of(x)));
+  return {values, scales, sum.defined() ? std::optional<at::Tensor>(sum) : std::nullopt};
+}
+
+// ---- learned relative position bias ------------------------------------------------------------------------------------
+struct EdgePositionBiasBackward : public torch::autograd::Node {
+  SavedVariable buckets;      // int16, -1: an edge without one
+  int64_t n_buckets = 0;
+
+  variable_list apply(variable_list&& grads) override {
+    return reporting([&] { return backward(grads); });
+  }
+  variable_list backward(const variable_list& grads) {
+    if (!grads[0].defined()) return variable_list(1);
+    const at::Tensor of = buckets.unpack();
+    const int64_t edges = of.numel(), heads = grads[0].size(-1);
+    // a second-order gradient is wanted, or many gradients at once (is_grads_batched)
+    if (at::GradMode::is_enabled() || at::isTensorSubclassLike(grads[0])) {
+      const at::Tensor known = of.ge(0).unsqueeze(-1), d = at::where(known, grads[0], at::zeros_like(grads[0]));
+      return {at::zeros({n_buckets, heads}, grads[0].options()).index_add(0, of.clamp_min(0).to(at::kLong), d)};
+    }
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(of.device());
+    const at::Tensor d = grads[0].contiguous(), dtable = at::empty({n_buckets, heads}, d.options());
+    size_t bytes = 0;
+    check(tgt_edge_position_bias_grad_scratch_bytes(edges, int(n_buckets), int(heads), &bytes));
+    const at::Tensor scratch = scratch_of(bytes, d);
+    check(tgt_edge_position_bias_grad(fptr(d), static_cast<const uint16_t*>(ptr(of)), edges, int(n_buckets), int(heads),
+                                      fptr(dtable), scratch.data_ptr(), scratch.numel(), stream_of(d)));
+    return {dtable};
+  }
+  std::string name() const override { return "EdgePositionBiasBackward"; }
+  void release_variables() override { buckets.reset_data(); }
+};
+
+// The caller has checked types, shapes and the borders.
+at::Tensor edge_position_bias(const at::Tensor& table, const at::Tensor& edge_index, const std::optional<at::Tensor>& positions,
+                              const std::vector<int32_t>& borders, bool both_ways) {
+  const at::Device device = table.device();
+  auto whole = [&](const at::Tensor& t) {
+    return t.is_cuda() && t.device() == device && (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt);
+  };
+  TORCH_CHECK(plain(table, device, at::kFloat) && table.dim() == 2 && whole(edge_index) && edge_index.dim() == 2 &&
+                  edge_index.size(0) == 2 && (!positions.has_value() || (whole(*positions) && positions->dim() == 1)) &&
+                  table.size(0) == int64_t(borders.size() + 1) * (both_ways ? 2 : 1),
+              "edge_position_bias: tensors that the kernels do not cover");
+  const c10::cuda::CUDAGuard guard(device);
+  const int64_t edges = edge_index.size(1), heads = table.size(1);
+  const bool record = torch::autograd::compute_requires_grad(table);
+  at::Tensor bias, buckets;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor tc = table.contiguous(), ec = edge_index.contiguous();
+    const at::Tensor pc = positions.has_value() ? positions->contiguous() : at::Tensor();
+    bias = at::empty({edges, heads}, table.options());
+    if (record) buckets = at::empty({edges}, table.options().dtype(at::kShort));
+    // no nodes: every id is outside, which takes a pointer to tell
+    const void* where = pc.defined() ? (pc.numel() > 0 ? pc.data_ptr() : static_cast<const void*>(tc.data_ptr())) : nullptr;
+    check(tgt_edge_position_bias(ptr(ec), edges, ec.scalar_type() == at::kLong, where, pc.defined() ? pc.numel() : 0,
+                                 pc.defined() && pc.scalar_type() == at::kLong, borders.data(), int(borders.size()), both_ways,
+                                 fptr(tc), int(heads), fptr(bias), static_cast<uint16_t*>(ptr(buckets)), stream_of(table)));
+  }
+  if (record) {
+    auto node = std::shared_ptr<EdgePositionBiasBackward>(new EdgePositionBiasBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(table));
+    node->buckets = SavedVariable(buckets, false);
+    node->n_buckets = table.size(0);
+    torch::autograd::set_history(bias, node);
+  }
+  return bias;
+}
+
+}  // namespace
+
+void bind_block(pybind11::module_& m) {
+  m.def("rms_norm_covers", &rms_norm_covers);
+  m.def("add_rms_norm", &add_rms_norm, Unlocked());
+  m.def("rms_norm_e4m3", &rms_norm_e4m3, Unlocked());
+  m.def("edge_position_bias", &edge_position_bias, Unlocked());
+}
+
+}  // namespace tgt_host

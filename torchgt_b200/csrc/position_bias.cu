@@ -1,0 +1,268 @@
+// Learned relative position bias of the attention's edges: the bias that tgt_sparse_attn_fwd takes per edge and head, from a
+// table with a row per bucket of the distance between the edge's ends, and the gradient of the table.
+//
+//   offset = position[source] - position[destination];  bias[e] = table[bucket(offset)];  dtable[b] = sum of dbias[e] of b's edges
+//
+// A bucket is the number of borders that the distance reaches (both ways: the second half of the table is for sources
+// behind the destination).  Borders are whole numbers made by the caller, so no logarithm decides on which side of one a distance
+// lies.
+// Forward: a warp takes 32 edges, a lane finds one edge's bucket, then the warp writes the 32 rows of bias as one run.
+// Backward: a warp adds the rows of dbias to sums of its own in shared memory, one per bucket and lane: lanes are (edge of a
+// group, head), so no two of them share a word or a bank, and what a hub's bucket costs is what any costs.  The sums
+// of a CTA's warps and then of the CTAs are added in a fixed order: no atomics, the same bits every time.  Both directions are bound by the
+// ids and the rows of bias; the forward keeps the buckets, 2 bytes an edge in the place of the 16 of two ids.
+#include "tgt_common.cuh"
+
+namespace tgt {
+namespace {
+
+constexpr int kMostBuckets = 512, kMostHeads = 256;
+constexpr int kBiasThreads = 256;
+constexpr uint16_t kNoBucket = 0xffff;      // of an edge with an id outside the positions
+
+struct BiasFwd {
+  const void* source;          // ids
+  const void* destination;
+  const void* positions;       // may be null: the ids themselves
+  int64_t n_positions, n_edges;
+  const float* table;
+  float* bias;
+  uint16_t* buckets;           // may be null
+  int heads, behind;           // behind: the first bucket of sources behind the destination, or 0
+  int n_borders, search;       // search: the largest power of two up to n_borders, 0 without any
+  unsigned share;              // 2^22 / pieces of a row, rounded up
+  int32_t borders[kMostBuckets];
+};
+
+template <typename Id, typename Pos>
+__device__ __forceinline__ int bucket_of(const BiasFwd& p, const int32_t* borders, int64_t e) {
+  int64_t s = static_cast<const Id*>(p.source)[e], d = static_cast<const Id*>(p.destination)[e];
+  if (p.positions != nullptr) {
+    if (s < 0 || s >= p.n_positions || d < 0 || d >= p.n_positions) return kNoBucket;
+    s = __ldg(static_cast<const Pos*>(p.positions) + s);
+    d = __ldg(static_cast<const Pos*>(p.positions) + d);
+  }
+  // the difference of any two positions fits 64 bits without a sign
+  const uint64_t far = s > d ? (p.behind > 0 ? uint64_t(s) - uint64_t(d) : 0) : uint64_t(d) - uint64_t(s);
+  const int32_t distance = far > 0x7fffffffu ? 0x7fffffff : int32_t(far);
+  int n = 0;
+  for (int step = p.search; step > 0; step >>= 1)
+    if (n + step <= p.n_borders && borders[n + step - 1] <= distance) n += step;
+  return n + (s > d ? p.behind : 0);
+}
+
+template <typename Id, typename Pos, int VEC>
+__global__ void __launch_bounds__(kBiasThreads) position_bias_kernel(const __grid_constant__ BiasFwd p) {
+  __shared__ int32_t s_borders[kMostBuckets];
+  for (int i = threadIdx.x; i < p.n_borders; i += kBiasThreads) s_borders[i] = p.borders[i];
+  __syncthreads();
+  const int lane = threadIdx.x % 32, pieces = p.heads / VEC;
+  const int64_t warps = int64_t(gridDim.x) * (kBiasThreads / 32);
+  for (int64_t e0 = (int64_t(blockIdx.x) * (kBiasThreads / 32) + threadIdx.x / 32) * 32; e0 < p.n_edges; e0 += warps * 32) {
+    const int64_t e = e0 + lane;
+    int bucket = kNoBucket;
+    if (e < p.n_edges) {
+      bucket = bucket_of<Id, Pos>(p, s_borders, e);
+      if (p.buckets != nullptr) p.buckets[e] = uint16_t(bucket);
+    }
+    const int live = int(min(p.n_edges - e0, int64_t(32))) * pieces;
+    float* const out = p.bias + e0 * p.heads;
+    for (int i = 0; i < pieces; ++i) {
+      const int piece = i * 32 + lane;
+      const int of = int((unsigned(piece) * p.share) >> 22);
+      const int b = __shfl_sync(0xffffffffu, bucket, of);
+      if (piece >= live) continue;
+      const float nan = __int_as_float(0x7fffffff);
+      if constexpr (VEC == 4) {
+        float4 v = make_float4(nan, nan, nan, nan);
+        if (b != kNoBucket) v = __ldg(reinterpret_cast<const float4*>(p.table) + b * pieces + (piece - of * pieces));
+        reinterpret_cast<float4*>(out)[piece] = v;
+      } else {
+        out[piece] = b != kNoBucket ? __ldg(p.table + b * pieces + (piece - of * pieces)) : nan;
+      }
+    }
+  }
+}
+
+struct BiasBwd {
+  const float* dbias;
+  const uint16_t* buckets;
+  float* partial;              // [gridDim.x][n_buckets][heads]
+  int64_t n_edges;
+  int n_buckets, heads;
+};
+
+// HP: heads of a warp, a power of two; blockIdx.y picks which
+template <int HP>
+__global__ void __launch_bounds__(kBiasThreads) position_bias_grad_kernel(const BiasBwd p) {
+  extern __shared__ float s_sums[];                          // [warps][n_buckets][32]
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  float* const sums = s_sums + warp * p.n_buckets * 32;
+  for (int b = 0; b < p.n_buckets; ++b) sums[b * 32 + lane] = 0.f;
+  constexpr int kSlots = 32 / HP;                            // edges of a group
+  const int slot = lane / HP, h0 = blockIdx.y * 32, h = h0 + lane % HP;
+  const bool has_head = h < p.heads;
+  constexpr int kBatch = HP < 8 ? HP : 8;                    // rows in flight
+  for (int64_t e0 = (int64_t(blockIdx.x) * warps + warp) * 32; e0 < p.n_edges; e0 += int64_t(gridDim.x) * warps * 32) {
+    const int bucket = e0 + lane < p.n_edges ? p.buckets[e0 + lane] : kNoBucket;
+#pragma unroll
+    for (int i0 = 0; i0 < HP; i0 += kBatch) {
+      float v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int64_t e = e0 + (i0 + i) * kSlots + slot;
+        v[i] = has_head && e < p.n_edges ? __ldg(p.dbias + e * p.heads + h) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int b = __shfl_sync(0xffffffffu, bucket, (i0 + i) * kSlots + slot);
+        if (b != kNoBucket) sums[b * 32 + lane] += v[i];
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.n_buckets * HP; i += blockDim.x) {
+    const int b = i / HP, head = i % HP;
+    if (h0 + head >= p.heads) continue;
+    float s = 0.f;
+    for (int w = 0; w < warps; ++w)
+#pragma unroll
+      for (int k = 0; k < kSlots; ++k) s += s_sums[(w * p.n_buckets + b) * 32 + k * HP + head];
+    p.partial[(int64_t(blockIdx.x) * p.n_buckets + b) * p.heads + h0 + head] = s;
+  }
+}
+
+__global__ void __launch_bounds__(kPartialSumThreads) position_bias_table_kernel(const float* partial, int n_parts, int values,
+                                                                                 float* dtable) {
+  __shared__ float s_part[16][32];
+  const int i = blockIdx.x * 32 + threadIdx.x % 32;
+  const float s = sum_partials(partial, n_parts, values, i, i < values, s_part);
+  if (threadIdx.x < 32 && i < values) dtable[i] = s;
+}
+
+struct GradPlan {
+  int hp, warps, smem, ctas;
+};
+constexpr int kMostSmem = 200 * 1024;
+GradPlan plan_grad(int64_t n_edges, int n_buckets, int heads) {
+  GradPlan g;
+  g.hp = 1;
+  while (g.hp < 32 && g.hp < heads) g.hp *= 2;
+  const int per_warp = n_buckets * 128;
+  g.warps = kMostSmem / per_warp;
+  g.warps = g.warps > kBiasThreads / 32 ? kBiasThreads / 32 : g.warps;
+  g.smem = g.warps * per_warp;
+  int resident = kMostSmem / g.smem;
+  resident = resident > 6 ? 6 : resident;
+  // a CTA clears and adds up its sums: at least eight steps a warp before there is a second
+  const int64_t steps = (n_edges + 31) / 32, want = (steps + 8 * g.warps - 1) / (8 * g.warps);
+  const int64_t most = int64_t(sm_count()) * resident;
+  g.ctas = int(want < 1 ? 1 : want > most ? most : want);
+  return g;
+}
+
+template <int HP>
+int launch_grad(const BiasBwd& p, const GradPlan& g, cudaStream_t stream) {
+  const int rc = allow_shared_memory<position_bias_grad_kernel<HP>>(kMostSmem);
+  if (rc != TGT_OK) return rc;
+  position_bias_grad_kernel<HP><<<dim3(g.ctas, (p.heads + 31) / 32), g.warps * 32, g.smem, stream>>>(p);
+  return TGT_OK;
+}
+
+int check_sizes(int64_t n_edges, int n_buckets, int heads) {
+  TGT_CHECK_ARG(n_edges >= 0, "n_edges must be >= 0");
+  TGT_CHECK_ARG(n_buckets >= 1 && heads >= 1, "the table must have a bucket and a head");
+  if (n_buckets > kMostBuckets || heads > kMostHeads)
+    return set_error(TGT_ERR_UNSUPPORTED, "%d buckets of %d heads: at most %d of %d", n_buckets, heads, kMostBuckets, kMostHeads);
+  return TGT_OK;
+}
+
+template <typename Id, typename Pos>
+int launch_forward(const BiasFwd& p, cudaStream_t stream) {
+  const int64_t want = (p.n_edges + kBiasThreads - 1) / kBiasThreads, most = int64_t(sm_count()) * (2048 / kBiasThreads);
+  const unsigned grid = unsigned(want < most ? want : most);
+  if (p.heads % 4 == 0 && aligned16(p.table) && aligned16(p.bias))
+    position_bias_kernel<Id, Pos, 4><<<grid, kBiasThreads, 0, stream>>>(p);
+  else
+    position_bias_kernel<Id, Pos, 1><<<grid, kBiasThreads, 0, stream>>>(p);
+  TGT_CHECK_CUDA(cudaGetLastError());
+  return TGT_OK;
+}
+
+}  // namespace
+}  // namespace tgt
+
+extern "C" int tgt_edge_position_bias(const void* edge_index, int64_t n_edges, int wide_ids, const void* positions,
+                                      int64_t n_positions, int wide_positions, const int32_t* borders, int n_borders,
+                                      int both_ways, const float* table, int heads, float* bias, uint16_t* buckets,
+                                      void* stream_) {
+  using namespace tgt;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  TGT_CHECK_ARG(n_borders >= 0 && n_borders < kMostBuckets, "n_borders must be 0 to %d", kMostBuckets - 1);
+  const int rc = check_sizes(n_edges, (n_borders + 1) * (both_ways ? 2 : 1), heads);
+  if (rc != TGT_OK) return rc;
+  TGT_CHECK_ARG(n_borders == 0 || borders != nullptr, "borders is null");
+  for (int i = 0; i < n_borders; ++i)
+    TGT_CHECK_ARG(borders[i] >= (i > 0 ? borders[i - 1] : 1), "borders must be positive and in order");
+  TGT_CHECK_ARG(positions == nullptr || n_positions >= 0, "n_positions must be >= 0");
+  if (n_edges == 0) return TGT_OK;
+  TGT_CHECK_ARG(edge_index && table && bias, "edge_index, table and bias must not be null");
+  BiasFwd p{};
+  p.source = edge_index;
+  p.destination = static_cast<const char*>(edge_index) + n_edges * (wide_ids ? 8 : 4);
+  p.positions = positions;
+  p.n_positions = n_positions; p.n_edges = n_edges;
+  p.table = table; p.bias = bias; p.buckets = buckets;
+  p.heads = heads;
+  p.behind = both_ways ? n_borders + 1 : 0;
+  p.n_borders = n_borders;
+  p.search = n_borders > 0 ? 1 : 0;
+  while (2 * p.search <= n_borders && p.search > 0) p.search *= 2;
+  const int pieces = heads % 4 == 0 && aligned16(table) && aligned16(bias) ? heads / 4 : heads;
+  p.share = ((1u << 22) + pieces - 1) / pieces;
+  for (int i = 0; i < n_borders; ++i) p.borders[i] = borders[i];
+  if (wide_ids)
+    return wide_positions ? launch_forward<int64_t, int64_t>(p, stream) : launch_forward<int64_t, int32_t>(p, stream);
+  return wide_positions ? launch_forward<int32_t, int64_t>(p, stream) : launch_forward<int32_t, int32_t>(p, stream);
+}
+
+extern "C" int tgt_edge_position_bias_grad_scratch_bytes(int64_t n_edges, int n_buckets, int heads, size_t* bytes) {
+  using namespace tgt;
+  TGT_CHECK_ARG(bytes != nullptr, "bytes is null");
+  const int rc = check_sizes(n_edges, n_buckets, heads);
+  if (rc != TGT_OK) return rc;
+  *bytes = size_t(plan_grad(n_edges, n_buckets, heads).ctas) * n_buckets * heads * sizeof(float);
+  return TGT_OK;
+}
+
+extern "C" int tgt_edge_position_bias_grad(const float* dbias, const uint16_t* buckets, int64_t n_edges, int n_buckets, int heads,
+                                           float* dtable, void* scratch, size_t scratch_bytes, void* stream_) {
+  using namespace tgt;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int rc = check_sizes(n_edges, n_buckets, heads);
+  if (rc != TGT_OK) return rc;
+  TGT_CHECK_ARG(dtable != nullptr, "dtable must not be null");
+  const int values = n_buckets * heads;
+  if (n_edges == 0) {
+    TGT_CHECK_CUDA(cudaMemsetAsync(dtable, 0, size_t(values) * sizeof(float), stream));
+    return TGT_OK;
+  }
+  TGT_CHECK_ARG(dbias && buckets, "dbias and buckets must not be null");
+  const GradPlan g = plan_grad(n_edges, n_buckets, heads);
+  const size_t need = size_t(g.ctas) * values * sizeof(float);
+  if (scratch == nullptr || scratch_bytes < need)
+    return set_error(TGT_ERR_WORKSPACE, "scratch holds %zu bytes, %zu needed", scratch_bytes, need);
+  const BiasBwd p{dbias, buckets, static_cast<float*>(scratch), n_edges, n_buckets, heads};
+  switch (g.hp) {
+    case 1: rc = launch_grad<1>(p, g, stream); break;
+    case 2: rc = launch_grad<2>(p, g, stream); break;
+    case 4: rc = launch_grad<4>(p, g, stream); break;
+    case 8: rc = launch_grad<8>(p, g, stream); break;
+    case 16: rc = launch_grad<16>(p, g, stream); break;
+    default: rc = launch_grad<32>(p, g, stream); break;
+  }
+  if (rc != TGT_OK) return rc;
+  position_bias_table_kernel<<<(values + 31) / 32, kPartialSumThreads, 0, stream>>>(p.partial, g.ctas, values, dtable);
+  TGT_CHECK_CUDA(cudaGetLastError());
+  return TGT_OK;
+}
