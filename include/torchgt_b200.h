@@ -528,6 +528,7 @@ TGT_API int tgt_linear_input_grad(const float* dy, const float* w, int64_t rows,
 #define TGT_ACT_NONE 0
 #define TGT_ACT_RELU 1
 #define TGT_ACT_GELU 2
+#define TGT_ACT_SILU 3   /* of the gated block only */
 TGT_API int tgt_linear_rows_multi(const float* a, const float* const* w, const float* const* bias, int count,
                                   int64_t rows, int reduce, int cols, int act, float* pre, const float* add,
                                   float* const* c, void* stream);
@@ -597,6 +598,34 @@ TGT_API int tgt_edge_position_bias(const void* edge_index, int64_t n_edges, int 
 TGT_API int tgt_edge_position_bias_grad_scratch_bytes(int64_t n_edges, int n_buckets, int heads, size_t* bytes);
 TGT_API int tgt_edge_position_bias_grad(const float* dbias, const uint16_t* buckets, int64_t n_edges, int n_buckets, int heads,
                                         float* dtable, void* scratch, size_t scratch_bytes, void* stream);
+
+/*
+ * Gated feed-forward block, h = act(x w_gate^T) * (x w_up^T), y = h w_down^T + add, and its gradients, with act TGT_ACT_SILU,
+ * TGT_ACT_GELU (exact) or TGT_ACT_RELU; w_gate and w_up are [mid, in], w_down is [out, mid], all tensors packed and of `dtype`,
+ * 16-byte aligned.  TGT_BF16: products on the tensor cores with fp32 sums, the activation and the product of the two
+ * projections in fp32 before h is rounded; widths multiples of 8, at most 65536.  TGT_F32: the products of tgt_linear_rows
+ * and what follows in a kernel of its own; in and mid multiples of 64, out of 4, at most 1024 (TGT_ERR_UNSUPPORTED otherwise).
+ *   hidden:      h, and where gate is not NULL (TGT_F32: never) gate = x w_gate^T and up = x w_up^T as the gradients need them
+ *   output:      y; add [rows, out] may be NULL and must not overlap y
+ *   hidden_grad: from dy [rows, out], dh = dy w_down: dgate = dh up act'(gate) and dup = dh act(gate)
+ *   input_grad:  dx = dgate w_gate + dup w_up
+ *   weight_grad: dw[i] [out_features, in_features] = dy[i]^T x for `count` 1 or 2 (host arrays of pointers): (dgate, dup) with x,
+ *                or dy with h.  Fixed order of summation; scratch holds parts of the sums.
+ * Waits are bounded as those of tgt_linear_rows are, and reported the same way.
+ */
+TGT_API int tgt_gated_hidden(const void* x, const void* w_gate, const void* w_up, int64_t rows, int in, int mid, int act,
+                             int dtype, void* h, void* gate, void* up, void* stream);
+TGT_API int tgt_gated_output(const void* h, const void* w_down, const void* add, int64_t rows, int mid, int out, int dtype,
+                             void* y, void* stream);
+TGT_API int tgt_gated_hidden_grad(const void* dy, const void* w_down, const void* gate, const void* up, int64_t rows, int out,
+                                  int mid, int act, int dtype, void* dgate, void* dup, void* stream);
+TGT_API int tgt_gated_input_grad(const void* dgate, const void* dup, const void* w_gate, const void* w_up, int64_t rows, int mid,
+                                 int in, int dtype, void* dx, void* stream);
+TGT_API int tgt_gated_weight_grad_scratch_bytes(int count, int64_t rows, int out_features, int in_features, int dtype,
+                                                size_t* bytes);
+TGT_API int tgt_gated_weight_grad(const void* const* dy, const void* x, int count, int64_t rows, int out_features,
+                                  int in_features, int dtype, void* const* dw, void* scratch, size_t scratch_bytes,
+                                  void* stream);
 
 #ifdef __cplusplus
 }

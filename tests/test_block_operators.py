@@ -81,3 +81,36 @@ def test_argument_checks_run_before_any_cuda_call():
     assert lib.tgt_edge_position_bias(None, 0, 1, None, 0, 0, borders, 3, 1, None, 257, None, None, None) == 3
     assert lib.tgt_edge_position_bias_grad_scratch_bytes(10, 513, 8, ctypes.byref(n)) == 3
     assert lib.tgt_edge_position_bias_grad(None, None, 1, 32, 8, None, None, 0, None) == 1
+
+
+def test_gated_block_arguments():
+    from torchgt_b200 import GatedFeedForward, _cabi, gated_feed_forward
+    x, wg, wu, wd = torch.randn(5, 64), torch.randn(96, 64), torch.randn(96, 64), torch.randn(64, 96)
+    want = (torch.nn.functional.silu(x @ wg.t()) * (x @ wu.t())) @ wd.t()
+    torch.testing.assert_close(gated_feed_forward(x, wg, wu, wd), want)
+    torch.testing.assert_close(gated_feed_forward(x, wg, wu, wd, residual=x), want + x)
+    for bad in ((x, wg, wu[:50], wd), (x, wg, wu, wd.t()), (x[:, :32], wg, wu, wd), (x, wg[0], wu, wd)):
+        with pytest.raises(ValueError):
+            gated_feed_forward(*bad)
+    with pytest.raises(ValueError):
+        gated_feed_forward(x, wg, wu, wd, "tanh")
+    with pytest.raises(ValueError):
+        gated_feed_forward(x, wg, wu, wd, "silu", x[0])
+    with pytest.raises(ValueError):
+        GatedFeedForward(64, 96, "tanh")
+    lib, n = _cabi.load(), ctypes.c_size_t()
+    hidden = lambda rows, i, m, act, dtype: lib.tgt_gated_hidden(None, None, None, rows, i, m, act, dtype, None, None, None, None)  # noqa: E731
+    assert hidden(0, 64, 64, 3, 1) == 0 and hidden(1, 64, 64, 3, 1) == 1 and hidden(-1, 64, 64, 3, 1) == 1
+    assert hidden(1, 64, 64, 0, 1) == 1 and hidden(1, 64, 64, 3, 7) == 1 and hidden(1, 0, 64, 3, 1) == 1
+    assert hidden(1, 60, 64, 3, 1) == 3 and hidden(1, 64, 65544, 3, 1) == 3 and hidden(2 ** 31, 64, 64, 3, 1) == 3
+    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 1, 24, None, None, None) == 1        # alignment
+    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 1, 16, 16, None, None) == 1          # gate without up
+    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 0, 16, None, None, None) == 1        # fp32 needs both
+    assert lib.tgt_gated_output(None, None, None, 1, 64, 64, 1, None, None) == 1
+    assert lib.tgt_gated_hidden_grad(None, None, None, None, 1, 64, 64, 3, 1, None, None, None) == 1
+    assert lib.tgt_gated_input_grad(None, None, None, None, 1, 64, 64, 1, None, None) == 1
+    assert lib.tgt_gated_weight_grad_scratch_bytes(3, 1, 64, 64, 1, ctypes.byref(n)) == 1
+    assert lib.tgt_gated_weight_grad_scratch_bytes(1, 1, 64, 60, 1, ctypes.byref(n)) == 3
+    assert lib.tgt_gated_weight_grad_scratch_bytes(2, 0, 64, 64, 1, ctypes.byref(n)) == 0 and n.value == 0
+    dw = (ctypes.c_void_p * 2)(16, 16)
+    assert lib.tgt_gated_weight_grad(None, None, 2, 1, 64, 64, 1, dw, None, 0, None) == 1

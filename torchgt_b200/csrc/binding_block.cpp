@@ -213,6 +213,159 @@ at::Tensor edge_position_bias(const at::Tensor& table, const at::Tensor& edge_in
   return bias;
 }
 
+// ---- gated feed-forward block -------------------------------------------------------------------------------------------
+// act(x w_gate^T) * (x w_up^T) times w_down^T, plus a residual.
+int activation_code(const std::string& name) {
+  TORCH_CHECK(name == "silu" || name == "gelu" || name == "relu", "gated_feed_forward knows silu, gelu and relu, not ", name);
+  return name == "silu" ? TGT_ACT_SILU : name == "gelu" ? TGT_ACT_GELU : TGT_ACT_RELU;
+}
+
+// contiguous, and copied when it is a view that starts off a 16-byte boundary (the kernels move 16 bytes at a time)
+at::Tensor kernel_ready(const at::Tensor& t) {
+  const at::Tensor c = t.contiguous();
+  return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0 ? c : c.clone();
+}
+
+struct GatedFeedForwardBackward : public torch::autograd::Node {
+  SavedVariable x, w_gate, w_up, w_down, hidden, gate, up;
+  int act = TGT_ACT_SILU;
+  bool with_residual = false;
+
+  variable_list apply(variable_list&& grads) override {
+    return reporting([&] { return backward(grads); });
+  }
+  // With create_graph the gradient is itself differentiated, with is_grads_batched there are many: the formula as operations.
+  variable_list recorded(const at::Tensor& dy, const at::Tensor& x_, const at::Tensor& wg, const at::Tensor& wu,
+                         const at::Tensor& wd) {
+    const at::Tensor g = at::matmul(x_, wg.t()), u = at::matmul(x_, wu.t()), dh = at::matmul(dy, wd);
+    at::Tensor a, slope;
+    if (act == TGT_ACT_RELU) {
+      a = at::relu(g);
+      slope = (g > 0).to(g.scalar_type());
+    } else if (act == TGT_ACT_GELU) {
+      a = at::gelu(g);
+      slope = at::gelu_backward(at::ones_like(g), g);
+    } else {
+      const at::Tensor s = at::sigmoid(g);
+      a = g * s;
+      slope = s * (1 + g * (1 - s));
+    }
+    auto flat = [](const at::Tensor& t) { return t.reshape({-1, t.size(-1)}); };
+    const at::Tensor dg = dh * u * slope, du = dh * a;
+    return {at::matmul(dg, wg) + at::matmul(du, wu), at::matmul(flat(dg).t(), flat(x_)), at::matmul(flat(du).t(), flat(x_)),
+            at::matmul(flat(dy).t(), flat(a * u)), with_residual ? dy : at::Tensor()};
+  }
+  variable_list backward(const variable_list& grads) {
+    variable_list result(5);
+    if (!grads[0].defined()) return result;
+    const at::Tensor x_ = x.unpack(), wg = w_gate.unpack(), wu = w_up.unpack(), wd = w_down.unpack();
+    if (at::GradMode::is_enabled() || at::isTensorSubclassLike(grads[0])) return recorded(grads[0], x_, wg, wu, wd);
+    if (with_residual) result[4] = grads[0];
+    const at::Tensor h = hidden.unpack(), g = gate.unpack(), u = up.unpack();
+    const c10::cuda::CUDAGuard guard(x_.device());
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t in = wg.size(1), mid = wg.size(0), out = wd.size(0), rows = x_.numel() / in;
+    const int type = type_code(x_);
+    const at::Tensor dy = kernel_ready(grads[0]);
+    void* const stream = stream_of(x_);
+    auto weight_gradients = [&](const std::vector<at::Tensor>& d, const at::Tensor& of, int64_t n, int64_t k, at::Tensor* dw) {
+      const void* from[2];
+      void* to[2];
+      for (size_t i = 0; i < d.size(); ++i) {
+        dw[i] = at::empty({n, k}, x_.options());
+        from[i] = ptr(d[i]);
+        to[i] = dw[i].data_ptr();
+      }
+      size_t bytes = 0;
+      check(tgt_gated_weight_grad_scratch_bytes(int(d.size()), rows, int(n), int(k), type, &bytes));
+      const at::Tensor scratch = scratch_of(bytes, x_);
+      check(tgt_gated_weight_grad(from, ptr(of), int(d.size()), rows, int(n), int(k), type, to, scratch.data_ptr(), scratch.numel(),
+                                  stream));
+    };
+    if (task_should_compute_output(3)) weight_gradients({dy}, h, out, mid, &result[3]);
+    const bool first = task_should_compute_output(1) || task_should_compute_output(2);
+    if (!first && !task_should_compute_output(0)) return result;
+    const at::Tensor dg = at::empty_like(g), du = at::empty_like(u);
+    const at::Tensor wdc = kernel_ready(wd);
+    check(tgt_gated_hidden_grad(ptr(dy), ptr(wdc), ptr(g), ptr(u), rows, int(out), int(mid), act, type, ptr(dg), ptr(du), stream));
+    if (first) weight_gradients({dg, du}, kernel_ready(x_), mid, in, &result[1]);
+    if (task_should_compute_output(0)) {
+      const at::Tensor wgc = kernel_ready(wg), wuc = kernel_ready(wu);
+      result[0] = at::empty(x_.sizes(), x_.options());
+      check(tgt_gated_input_grad(ptr(dg), ptr(du), ptr(wgc), ptr(wuc), rows, int(mid), int(in), type, ptr(result[0]), stream));
+    }
+    return result;
+  }
+  std::string name() const override { return "GatedFeedForwardBackward"; }
+  void release_variables() override {
+    for (SavedVariable* v : {&x, &w_gate, &w_up, &w_down, &hidden, &gate, &up}) v->reset_data();
+  }
+};
+
+bool gated_feed_forward_covers(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
+                               const std::optional<at::Tensor>& residual) {
+  if (!x.defined() || at::isTensorSubclassLike(x) || !kernel_type(x.scalar_type()) || x.dim() < 1) return false;
+  for (const at::Tensor* t : {&x, &wg, &wu, &wd})
+    if (!plain(*t, x.device(), x.scalar_type())) return false;
+  if (wg.dim() != 2 || wd.dim() != 2 || wu.sizes() != wg.sizes() || wd.size(1) != wg.size(0) || x.size(-1) != wg.size(1)) return false;
+  const int64_t in = wg.size(1), mid = wg.size(0), out = wd.size(0);
+  if (in < 1 || mid < 1 || out < 1) return false;
+  if (x.scalar_type() == at::kFloat) {
+    if (in % 64 != 0 || mid % 64 != 0 || out % 4 != 0 || in > 1024 || mid > 1024 || out > 1024) return false;
+  } else if (in % 8 != 0 || mid % 8 != 0 || out % 8 != 0 || in > 65536 || mid > 65536 || out > 65536 ||
+             x.numel() / in > (int64_t(1) << 30)) {
+    return false;
+  }
+  if (!residual.has_value()) return true;
+  auto sizes = x.sizes().vec();
+  sizes.back() = out;
+  return plain(*residual, x.device(), x.scalar_type()) && residual->sizes() == at::IntArrayRef(sizes);
+}
+
+at::Tensor gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
+                              const std::string& activation, const std::optional<at::Tensor>& residual_in) {
+  const int act = activation_code(activation);
+  TORCH_CHECK(gated_feed_forward_covers(x, wg, wu, wd, residual_in), "gated_feed_forward: tensors that the kernels do not cover");
+  const at::Tensor residual = residual_in.value_or(at::Tensor());
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t in = wg.size(1), mid = wg.size(0), out = wd.size(0), rows = x.numel() / in;
+  const int type = type_code(x);
+  const bool record = torch::autograd::compute_requires_grad(x, wg, wu, wd, residual);
+  at::Tensor y, h, g, u;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor xc = kernel_ready(x), wgc = kernel_ready(wg), wuc = kernel_ready(wu), wdc = kernel_ready(wd),
+                     rc = residual.defined() ? kernel_ready(residual) : residual;
+    auto sizes = x.sizes().vec();
+    sizes.back() = mid;
+    h = at::empty(sizes, x.options());
+    if (record || type == TGT_F32) {
+      g = at::empty(sizes, x.options());
+      u = at::empty(sizes, x.options());
+    }
+    sizes.back() = out;
+    y = at::empty(sizes, x.options());
+    void* const stream = stream_of(x);
+    check(tgt_gated_hidden(ptr(xc), ptr(wgc), ptr(wuc), rows, int(in), int(mid), act, type, ptr(h), ptr(g), ptr(u), stream));
+    check(tgt_gated_output(ptr(h), ptr(wdc), ptr(rc), rows, int(mid), int(out), type, ptr(y), stream));
+  }
+  if (record) {
+    auto node = std::shared_ptr<GatedFeedForwardBackward>(new GatedFeedForwardBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, wg, wu, wd, residual));
+    node->act = act;
+    node->with_residual = residual.defined();
+    node->x = SavedVariable(x, false);
+    node->w_gate = SavedVariable(wg, false);
+    node->w_up = SavedVariable(wu, false);
+    node->w_down = SavedVariable(wd, false);
+    node->hidden = SavedVariable(h, false);
+    node->gate = SavedVariable(g, false);
+    node->up = SavedVariable(u, false);
+    torch::autograd::set_history(y, node);
+  }
+  return y;
+}
+
 }  // namespace
 
 void bind_block(pybind11::module_& m) {
@@ -220,6 +373,8 @@ void bind_block(pybind11::module_& m) {
   m.def("add_rms_norm", &add_rms_norm, Unlocked());
   m.def("rms_norm_e4m3", &rms_norm_e4m3, Unlocked());
   m.def("edge_position_bias", &edge_position_bias, Unlocked());
+  m.def("gated_feed_forward_covers", &gated_feed_forward_covers);
+  m.def("gated_feed_forward", &gated_feed_forward, Unlocked());
 }
 
 }  // namespace tgt_host
