@@ -605,20 +605,24 @@ TGT_API int tgt_edge_position_bias_grad(const float* dbias, const uint16_t* buck
  * 16-byte aligned.  TGT_BF16: products on the tensor cores with fp32 sums, the activation and the product of the two
  * projections in fp32 before h is rounded; widths multiples of 8, at most 65536.  TGT_F32: the products of tgt_linear_rows
  * and what follows in a kernel of its own; in and mid multiples of 64, out of 4, at most 1024 (TGT_ERR_UNSUPPORTED otherwise).
- *   hidden:      h, and where gate is not NULL (TGT_F32: never) gate = x w_gate^T and up = x w_up^T as the gradients need them
+ *   hidden:      h, and where gate is not NULL (TGT_F32: never) gate = x w_gate^T and up = x w_up^T as the gradients need them:
+ *                in bf16 the upper 16 bits of their fp32 sums, and in low [rows, mid] the next 8 bits of both (gate's in the
+ *                lower byte); in fp32 the sums, and low is not used
  *   output:      y; add [rows, out] may be NULL and must not overlap y
  *   hidden_grad: from dy [rows, out], dh = dy w_down: dgate = dh up act'(gate) and dup = dh act(gate)
  *   input_grad:  dx = dgate w_gate + dup w_up
  *   weight_grad: dw[i] [out_features, in_features] = dy[i]^T x for `count` 1 or 2 (host arrays of pointers): (dgate, dup) with x,
- *                or dy with h.  Fixed order of summation; scratch holds parts of the sums.
+ *                or dy with h
+ * Sums have a fixed order; scratch (16-byte aligned, may be NULL where tgt_gated_weight_grad_scratch_bytes says 0) holds parts
+ * of them.
  * Waits are bounded as those of tgt_linear_rows are, and reported the same way.
  */
 TGT_API int tgt_gated_hidden(const void* x, const void* w_gate, const void* w_up, int64_t rows, int in, int mid, int act,
-                             int dtype, void* h, void* gate, void* up, void* stream);
+                             int dtype, void* h, void* gate, void* up, void* low, void* stream);
 TGT_API int tgt_gated_output(const void* h, const void* w_down, const void* add, int64_t rows, int mid, int out, int dtype,
                              void* y, void* stream);
-TGT_API int tgt_gated_hidden_grad(const void* dy, const void* w_down, const void* gate, const void* up, int64_t rows, int out,
-                                  int mid, int act, int dtype, void* dgate, void* dup, void* stream);
+TGT_API int tgt_gated_hidden_grad(const void* dy, const void* w_down, const void* gate, const void* up, const void* low,
+                                  int64_t rows, int out, int mid, int act, int dtype, void* dgate, void* dup, void* stream);
 TGT_API int tgt_gated_input_grad(const void* dgate, const void* dup, const void* w_gate, const void* w_up, int64_t rows, int mid,
                                  int in, int dtype, void* dx, void* stream);
 TGT_API int tgt_gated_weight_grad_scratch_bytes(int count, int64_t rows, int out_features, int in_features, int dtype,

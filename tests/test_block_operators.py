@@ -99,15 +99,16 @@ def test_gated_block_arguments():
     with pytest.raises(ValueError):
         GatedFeedForward(64, 96, "tanh")
     lib, n = _cabi.load(), ctypes.c_size_t()
-    hidden = lambda rows, i, m, act, dtype: lib.tgt_gated_hidden(None, None, None, rows, i, m, act, dtype, None, None, None, None)  # noqa: E731
+    hidden = lambda rows, i, m, act, dtype: lib.tgt_gated_hidden(None, None, None, rows, i, m, act, dtype, None, None, None, None, None)  # noqa: E731
     assert hidden(0, 64, 64, 3, 1) == 0 and hidden(1, 64, 64, 3, 1) == 1 and hidden(-1, 64, 64, 3, 1) == 1
     assert hidden(1, 64, 64, 0, 1) == 1 and hidden(1, 64, 64, 3, 7) == 1 and hidden(1, 0, 64, 3, 1) == 1
     assert hidden(1, 60, 64, 3, 1) == 3 and hidden(1, 64, 65544, 3, 1) == 3 and hidden(2 ** 31, 64, 64, 3, 1) == 3
-    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 1, 24, None, None, None) == 1        # alignment
-    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 1, 16, 16, None, None) == 1          # gate without up
-    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 0, 16, None, None, None) == 1        # fp32 needs both
+    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 1, 24, None, None, None, None) == 1        # alignment
+    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 1, 16, 16, None, 16, None) == 1          # gate without up
+    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 1, 16, 16, 16, None, None) == 1          # without the bits below
+    assert lib.tgt_gated_hidden(16, 16, 16, 1, 64, 64, 3, 0, 16, None, None, None, None) == 1        # fp32 needs both
     assert lib.tgt_gated_output(None, None, None, 1, 64, 64, 1, None, None) == 1
-    assert lib.tgt_gated_hidden_grad(None, None, None, None, 1, 64, 64, 3, 1, None, None, None) == 1
+    assert lib.tgt_gated_hidden_grad(None, None, None, None, None, 1, 64, 64, 3, 1, None, None, None) == 1
     assert lib.tgt_gated_input_grad(None, None, None, None, 1, 64, 64, 1, None, None) == 1
     assert lib.tgt_gated_weight_grad_scratch_bytes(3, 1, 64, 64, 1, ctypes.byref(n)) == 1
     assert lib.tgt_gated_weight_grad_scratch_bytes(1, 1, 64, 60, 1, ctypes.byref(n)) == 3

@@ -156,9 +156,9 @@ SIGNATURES = {
     "tgt_edge_position_bias_grad_scratch_bytes": (c_int, [c_int64, c_int, c_int, POINTER(c_size_t)]),
     "tgt_edge_position_bias_grad": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "tgt_gated_hidden": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
-                                 c_void_p]),
+                                 c_void_p, c_void_p]),
     "tgt_gated_output": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p]),
-    "tgt_gated_hidden_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p,
+    "tgt_gated_hidden_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p,
                                       c_void_p, c_void_p]),
     "tgt_gated_input_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p]),
     "tgt_gated_weight_grad_scratch_bytes": (c_int, [c_int, c_int64, c_int, c_int, c_int, POINTER(c_size_t)]),

@@ -227,7 +227,7 @@ at::Tensor kernel_ready(const at::Tensor& t) {
 }
 
 struct GatedFeedForwardBackward : public torch::autograd::Node {
-  SavedVariable x, w_gate, w_up, w_down, hidden, gate, up;
+  SavedVariable x, w_gate, w_up, w_down, hidden, gate, up, low;   // low: of bf16 (tgt_gated_hidden)
   int act = TGT_ACT_SILU;
   bool with_residual = false;
 
@@ -261,7 +261,7 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
     const at::Tensor x_ = x.unpack(), wg = w_gate.unpack(), wu = w_up.unpack(), wd = w_down.unpack();
     if (at::GradMode::is_enabled() || at::isTensorSubclassLike(grads[0])) return recorded(grads[0], x_, wg, wu, wd);
     if (with_residual) result[4] = grads[0];
-    const at::Tensor h = hidden.unpack(), g = gate.unpack(), u = up.unpack();
+    const at::Tensor h = hidden.unpack(), g = gate.unpack(), u = up.unpack(), l = low.unpack();
     const c10::cuda::CUDAGuard guard(x_.device());
     const at::AutoDispatchBelowADInplaceOrView below;
     const int64_t in = wg.size(1), mid = wg.size(0), out = wd.size(0), rows = x_.numel() / in;
@@ -287,7 +287,7 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
     if (!first && !task_should_compute_output(0)) return result;
     const at::Tensor dg = at::empty_like(g), du = at::empty_like(u);
     const at::Tensor wdc = kernel_ready(wd);
-    check(tgt_gated_hidden_grad(ptr(dy), ptr(wdc), ptr(g), ptr(u), rows, int(out), int(mid), act, type, ptr(dg), ptr(du), stream));
+    check(tgt_gated_hidden_grad(ptr(dy), ptr(wdc), ptr(g), ptr(u), ptr(l), rows, int(out), int(mid), act, type, ptr(dg), ptr(du), stream));
     if (first) weight_gradients({dg, du}, kernel_ready(x_), mid, in, &result[1]);
     if (task_should_compute_output(0)) {
       const at::Tensor wgc = kernel_ready(wg), wuc = kernel_ready(wu);
@@ -298,7 +298,7 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
   }
   std::string name() const override { return "GatedFeedForwardBackward"; }
   void release_variables() override {
-    for (SavedVariable* v : {&x, &w_gate, &w_up, &w_down, &hidden, &gate, &up}) v->reset_data();
+    for (SavedVariable* v : {&x, &w_gate, &w_up, &w_down, &hidden, &gate, &up, &low}) v->reset_data();
   }
 };
 
@@ -331,7 +331,7 @@ at::Tensor gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const a
   const int64_t in = wg.size(1), mid = wg.size(0), out = wd.size(0), rows = x.numel() / in;
   const int type = type_code(x);
   const bool record = torch::autograd::compute_requires_grad(x, wg, wu, wd, residual);
-  at::Tensor y, h, g, u;
+  at::Tensor y, h, g, u, l;
   {
     const at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor xc = kernel_ready(x), wgc = kernel_ready(wg), wuc = kernel_ready(wu), wdc = kernel_ready(wd),
@@ -342,11 +342,12 @@ at::Tensor gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const a
     if (record || type == TGT_F32) {
       g = at::empty(sizes, x.options());
       u = at::empty(sizes, x.options());
+      if (type == TGT_BF16) l = at::empty(sizes, x.options());
     }
     sizes.back() = out;
     y = at::empty(sizes, x.options());
     void* const stream = stream_of(x);
-    check(tgt_gated_hidden(ptr(xc), ptr(wgc), ptr(wuc), rows, int(in), int(mid), act, type, ptr(h), ptr(g), ptr(u), stream));
+    check(tgt_gated_hidden(ptr(xc), ptr(wgc), ptr(wuc), rows, int(in), int(mid), act, type, ptr(h), ptr(g), ptr(u), ptr(l), stream));
     check(tgt_gated_output(ptr(h), ptr(wdc), ptr(rc), rows, int(mid), int(out), type, ptr(y), stream));
   }
   if (record) {
@@ -361,6 +362,7 @@ at::Tensor gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const a
     node->hidden = SavedVariable(h, false);
     node->gate = SavedVariable(g, false);
     node->up = SavedVariable(u, false);
+    node->low = SavedVariable(l, false);
     torch::autograd::set_history(y, node);
   }
   return y;

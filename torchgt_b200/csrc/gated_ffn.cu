@@ -13,7 +13,7 @@
 namespace tgt {
 namespace tma {
 
-int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t columns, int box_rows, int box_columns) {
+int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t columns, int box_rows) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -27,11 +27,11 @@ int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t columns, 
     entry.store(f, std::memory_order_release);
   }
   const cuuint64_t sizes[2] = {cuuint64_t(columns), cuuint64_t(rows)}, pitch[1] = {cuuint64_t(columns) * 2};
-  const cuuint32_t box[2] = {cuuint32_t(box_columns), cuuint32_t(box_rows)}, steps[2] = {1, 1};
+  const cuuint32_t box[2] = {64, cuuint32_t(box_rows)}, steps[2] = {1, 1};
   auto encode = [&] {
     return reinterpret_cast<Encode>(f)(
         map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), sizes, pitch, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        box_columns == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult rc = encode();
@@ -56,11 +56,10 @@ constexpr int kMostWidth = 65536;
 constexpr int64_t kMostRows = int64_t(1) << 30;
 
 int operand(CUtensorMap* map, const void* base, int64_t rows, int64_t columns, bool mn_major, int tile_rows) {
-  return tma::make_map(map, base, rows, columns, mn_major ? gemm::kChunk : tile_rows, 64);
+  return tma::make_map(map, base, rows, columns, mn_major ? gemm::kChunk : tile_rows);
 }
-int result(CUtensorMap* map, const void* base, int64_t rows, int64_t columns) {
-  return tma::make_map(map, base, rows, columns, 32, gemm::kStoreCols);
-}
+uint16_t* words(void* t) { return static_cast<uint16_t*>(t); }
+const uint16_t* words(const void* t) { return static_cast<const uint16_t*>(t); }
 int tiles_of(int64_t n, int tile) { return int((n + tile - 1) / tile); }
 
 #define TGT_RETURN_IF(...)             \
@@ -69,58 +68,125 @@ int tiles_of(int64_t n, int tile) { return int((n + tile - 1) / tile); }
     if (_rc != TGT_OK) return _rc;     \
   } while (0)
 
-template <int BN, bool A_MN, bool B_MN, gemm::Finish FINISH>
-int launch(const Gemm& p, int grid, cudaStream_t stream) {
-  constexpr auto kernel = gemm::gemm_kernel<BN, A_MN, B_MN, FINISH>;
-  TGT_RETURN_IF(allow_shared_memory<gemm::gemm_kernel<BN, A_MN, B_MN, FINISH>>(gemm::smem_bytes(BN)));
-  kernel<<<grid, gemm::kThreads, gemm::smem_bytes(BN), stream>>>(p);
-  TGT_CHECK_CUDA(cudaGetLastError());
+// How a product is cut up: tiles of 128 rows of a CTA, or of 256 of a pair, x `bn` columns.
+struct Cut {
+  bool pair;
+  int bn;
+  int rows() const { return pair ? 2 * gemm::kTileM : gemm::kTileM; }
+  int b_rows() const { return pair ? bn / 2 : bn; }      // of B that one copy brings in
+};
+
+template <int BN, bool PAIR, bool A_MN, bool B_MN, gemm::Finish FINISH>
+int launch(const Gemm& p, int walkers, cudaStream_t stream) {
+  constexpr int kSmem = gemm::smem_bytes(PAIR ? BN / 2 : BN, FINISH);
+  TGT_RETURN_IF(allow_shared_memory<gemm::gemm_kernel<BN, PAIR, A_MN, B_MN, FINISH>>(kSmem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(walkers * (PAIR ? 2 : 1));
+  cfg.blockDim = dim3(gemm::kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  if (PAIR) {
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  TGT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm::gemm_kernel<BN, PAIR, A_MN, B_MN, FINISH>, p));
   return TGT_OK;
 }
 
-// Columns of a tile: the width whose rounds of tiles over the SMs cost least, a column of a narrower tile costing more (its
-// rows are read again, and products of fewer columns do not fill the tensor cores).
-int tile_columns_for(int64_t m, int columns, int narrowest) {
-  int best = 256;
+// Everything about how a product is done that its sizes decide.
+struct Plan {
+  Cut cut;
+  int m_tiles, n_tiles, product_tiles, chunks, walkers, whole;
+  int shared() const { return m_tiles * n_tiles - whole; }
+  size_t scratch() const { return shared() == 0 ? 0 : size_t(shared() + walkers) * cut.bn * cut.rows() * sizeof(float); }
+  void into(Gemm& p) const {
+    p.m_tiles = m_tiles; p.n_tiles = n_tiles; p.product_tiles = product_tiles;
+    p.chunks = chunks; p.whole = whole;
+  }
+};
+
+constexpr Cut kCuts[] = {{true, 256}, {true, 128}, {false, 256}, {false, 128}, {false, 64}};
+// The cut, and whether the last round's tiles are shared, of the least time by what was measured: us a chunk of k, a finish of
+// 256 columns, a start, and sharing.  us by pairs of 256 and 128 columns, single CTAs of 256, 128 and 64: y of 8,191 rows, 5,632 x 2,048
+// 137, 153, 187, 172, 307; 333 rows, 2,048 x 768 16.6, 12.6, 16.3, 13.7, 11.8; dx of 64,000 rows, 128 x 64 12.8, 11.9, 13.3, 10.0, 8.5;
+// h of 1,000 rows, 768 x 2,048, with what is kept 12.5, 14.6, 11.5, 13.0, -.  Shared or not: two weight gradients of 16,384 rows, 2,816 x
+// 1,024 135 / 166 (88 tiles for 74 pairs), of 64,000 rows, 128 x 64 19 / 223; one of 16,384 rows, 1,024 x 2,816 (44 tiles) 89 / 83.
+Plan plan_for(int products, int64_t m, int columns, int narrowest, int chunks, double finish, bool may_share) {
+  constexpr double kChunkTime[] = {0.39, 0.255, 0.42, 0.277, 0.235}, kStart[] = {1, 1, 0, 0, 0};
+  Plan best{};
   double least = 0;
-  for (int bn = 256; bn >= narrowest; bn /= 2) {
-    const int64_t tiles = int64_t(tiles_of(m, gemm::kTileM)) * tiles_of(columns, bn);
-    const int64_t rounds = (tiles + sm_count() - 1) / sm_count();
-    const double cost = double(rounds) * (bn == 256 ? 256 : bn == 128 ? 140 : 84);
-    if (bn == 256 || cost < least) {
-      best = bn;
-      least = cost;
+  for (int i = 0; i < 5; ++i) {
+    Plan q;
+    q.cut = kCuts[i];
+    if (q.cut.bn < narrowest) continue;
+    q.product_tiles = tiles_of(m, q.cut.rows());
+    q.m_tiles = q.product_tiles * products;
+    q.n_tiles = tiles_of(columns, q.cut.bn);
+    q.chunks = chunks;
+    const int64_t tiles = int64_t(q.m_tiles) * q.n_tiles, most = sm_count() / (q.cut.pair ? 2 : 1);
+    const double out = finish * q.cut.bn / 256;
+    for (int share = 0; share < (may_share ? 2 : 1); ++share) {
+      q.whole = int(share ? tiles / most * most : tiles);
+      const int64_t parts = q.shared() * int64_t(chunks);
+      if (share && (parts == 0 || (q.whole > 0 && parts < most))) continue;
+      q.walkers = int(share ? (q.whole > 0 || parts > most ? most : parts) : tiles < most ? tiles : most);
+      const int64_t rounds = (q.whole + most - 1) / most;
+      // SMs without a tile leave power to the others
+      const double chunk = kChunkTime[i] * (0.8 + 0.2 * (share || rounds == 0 ? 1.0 : double(q.whole) / double(rounds * most)));
+      const double round = chunks * chunk > out ? chunks * chunk : out;
+      double time = kStart[i] + out + double(rounds) * round;
+      // what is shared is read at other places of k by everybody; then the parts are written, read and added
+      if (share) time += double(parts) / q.walkers * chunk * 1.15 + 8 + double(q.scratch()) / 2e6;
+      if (least == 0 || time < least) {
+        best = q;
+        least = time;
+      }
     }
   }
   return best;
 }
-int grid_for(const Gemm& p) {
-  const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles;
-  return int(tiles < sm_count() ? tiles : sm_count());
+
+template <int BN, bool PAIR, bool A_MN, bool B_MN, gemm::Finish FINISH>
+int launch_cut(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+  if (q.scratch() > 0) {
+    if (scratch == nullptr || scratch_bytes < q.scratch())
+      return set_error(TGT_ERR_WORKSPACE, "scratch holds %zu bytes, %zu needed", scratch_bytes, q.scratch());
+    TGT_CHECK_ARG(aligned16(scratch), "scratch must be 16-byte aligned");
+    p.partial = static_cast<float*>(scratch);
+  }
+  TGT_RETURN_IF(launch<BN, PAIR, A_MN, B_MN, FINISH>(p, q.walkers, stream));
+  if constexpr (A_MN) {
+    if (q.shared() == 0) return TGT_OK;
+    const gemm::SumParts s{p.partial, {p.out[0], p.out[1]}, p.m, p.n, q.m_tiles, q.n_tiles,
+                           q.product_tiles, q.whole, q.chunks, q.walkers};
+    const dim3 grid(q.shared(), q.cut.rows() / 32 * BN / 64);
+    if (q.walkers / q.shared() > 8) gemm::sum_parts_kernel<BN, PAIR, 4><<<grid, 1024, 0, stream>>>(s);
+    else gemm::sum_parts_kernel<BN, PAIR, 1><<<grid, 256, 0, stream>>>(s);
+    TGT_CHECK_CUDA(cudaGetLastError());
+  }
+  return TGT_OK;
 }
 template <bool A_MN, bool B_MN, gemm::Finish FINISH>
-int launch_any(int bn, const Gemm& p, cudaStream_t stream) {
-  if (bn == 256) return launch<256, A_MN, B_MN, FINISH>(p, grid_for(p), stream);
-  if (bn == 128) return launch<128, A_MN, B_MN, FINISH>(p, grid_for(p), stream);
-  if constexpr (FINISH != gemm::kGated) return launch<64, A_MN, B_MN, FINISH>(p, grid_for(p), stream);
-  return set_error(TGT_ERR_INVALID, "no tile of %d columns", bn);
+int launch_plan(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+  q.into(p);
+  if (q.cut.pair) {
+    if (q.cut.bn == 256) return launch_cut<256, true, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
+    return launch_cut<128, true, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
+  }
+  if (q.cut.bn == 256) return launch_cut<256, false, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
+  if (q.cut.bn == 128) return launch_cut<128, false, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
+  if constexpr (FINISH != gemm::kGated) return launch_cut<64, false, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
+  return set_error(TGT_ERR_INVALID, "no tile of %d columns", q.cut.bn);
 }
 
-// What weight_grad's parts need: tiles of 128 rows of out_features x `bn` of in_features, `ctas` shares of all their chunks.
-struct PartsPlan {
-  int bn, product_tiles, m_tiles, n_tiles, chunks, ctas;
-  size_t bytes() const { return (size_t(m_tiles) * n_tiles + ctas) * bn * gemm::kTileM * sizeof(float); }
-};
-PartsPlan plan_parts(int count, int64_t rows, int out_features, int in_features) {
-  PartsPlan q;
-  q.bn = in_features > 128 ? 256 : in_features > 64 ? 128 : 64;
-  q.product_tiles = tiles_of(out_features, gemm::kTileM);
-  q.m_tiles = q.product_tiles * count;
-  q.n_tiles = tiles_of(in_features, q.bn);
-  q.chunks = tiles_of(rows, gemm::kChunk);
-  const int64_t all = int64_t(q.m_tiles) * q.n_tiles * q.chunks;
-  q.ctas = int(all < sm_count() ? all : sm_count());
-  return q;
+// the finishes' times of 256 columns (us)
+constexpr double kPlainTime = 3, kPlusTime = 4, kGatedTime = 3, kKeptTime = 4, kGradTime = 5;
+Plan weight_grad_plan(int count, int64_t rows, int out_features, int in_features) {
+  return plan_for(count, out_features, in_features, 64, tiles_of(rows, gemm::kChunk), kPlainTime, true);
 }
 
 int check_widths(int64_t rows, int a, int b, int dtype, int act) {
@@ -179,14 +245,16 @@ int gate_grid(int64_t n) {
 }  // namespace tgt
 
 extern "C" int tgt_gated_hidden(const void* x, const void* w_gate, const void* w_up, int64_t rows, int in, int mid, int act,
-                                int dtype, void* h, void* gate, void* up, void* stream_) {
+                                int dtype, void* h, void* gate, void* up, void* low, void* stream_) {
   using namespace tgt;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   TGT_RETURN_IF(check_widths(rows, in, mid, dtype, act));
-  TGT_CHECK_ARG((gate == nullptr) == (up == nullptr), "gate and up go together");
+  TGT_CHECK_ARG((gate == nullptr) == (up == nullptr) && (dtype == TGT_F32 || (gate == nullptr) == (low == nullptr)),
+                "gate, up and in bf16 low go together");
   if (rows == 0) return TGT_OK;
   TGT_CHECK_ARG(x && w_gate && w_up && h, "x, w_gate, w_up and h must not be null");
-  TGT_CHECK_ARG(aligned16(x) && aligned16(w_gate) && aligned16(w_up) && aligned16(h) && aligned16(gate) && aligned16(up),
+  TGT_CHECK_ARG(aligned16(x) && aligned16(w_gate) && aligned16(w_up) && aligned16(h) && aligned16(gate) && aligned16(up) &&
+                    aligned16(low),
                 "tensors must be 16-byte aligned");
   if (dtype == TGT_F32) {
     TGT_CHECK_ARG(gate != nullptr, "in fp32 gate and up must not be null");
@@ -203,22 +271,18 @@ extern "C" int tgt_gated_hidden(const void* x, const void* w_gate, const void* w
   }
   Gemm p{};
   TGT_RETURN_IF(expired_wait_word(&p.expired));
-  const int bn = tile_columns_for(rows, 2 * mid, 128);
+  const Plan q = plan_for(1, rows, 2 * mid, 128, tiles_of(in, gemm::kChunk), gate != nullptr ? kKeptTime : kGatedTime, false);
   TGT_RETURN_IF(operand(&p.a[0], x, rows, in, false, gemm::kTileM));
-  TGT_RETURN_IF(operand(&p.b[0], w_gate, mid, in, false, bn / 2));
-  TGT_RETURN_IF(operand(&p.b[1], w_up, mid, in, false, bn / 2));
+  TGT_RETURN_IF(operand(&p.b[0], w_gate, mid, in, false, q.cut.bn / 2));
+  TGT_RETURN_IF(operand(&p.b[1], w_up, mid, in, false, q.cut.bn / 2));
   p.a[1] = p.a[0];
-  TGT_RETURN_IF(result(&p.out[0], h, rows, mid));
+  p.out[0] = words(h);
   p.keep = gate != nullptr;
-  if (p.keep) {
-    TGT_RETURN_IF(result(&p.out[1], gate, rows, mid));
-    TGT_RETURN_IF(result(&p.out[2], up, rows, mid));
-  }
-  p.m = rows; p.n = mid;
-  p.m_tiles = tiles_of(rows, gemm::kTileM); p.n_tiles = tiles_of(mid, bn / 2);
-  p.chunks = p.source_chunks = tiles_of(in, gemm::kChunk);
+  p.out[1] = words(gate); p.out[2] = words(up); p.out[3] = words(low);
+  p.m = int(rows); p.n = mid;
+  p.source_chunks = q.chunks;
   p.act = act;
-  return launch_any<false, false, gemm::kGated>(bn, p, stream);
+  return launch_plan<false, false, gemm::kGated>(q, p, nullptr, 0, stream);
 }
 
 extern "C" int tgt_gated_output(const void* h, const void* w_down, const void* add, int64_t rows, int mid, int out, int dtype,
@@ -237,26 +301,28 @@ extern "C" int tgt_gated_output(const void* h, const void* w_down, const void* a
   }
   Gemm p{};
   TGT_RETURN_IF(expired_wait_word(&p.expired));
-  const int bn = tile_columns_for(rows, out, 64);
+  const Plan q = plan_for(1, rows, out, 64, tiles_of(mid, gemm::kChunk), add != nullptr ? kPlusTime : kPlainTime, false);
   TGT_RETURN_IF(operand(&p.a[0], h, rows, mid, false, gemm::kTileM));
-  TGT_RETURN_IF(operand(&p.b[0], w_down, out, mid, false, bn));
+  TGT_RETURN_IF(operand(&p.b[0], w_down, out, mid, false, q.cut.b_rows()));
   p.a[1] = p.a[0]; p.b[1] = p.b[0];
-  TGT_RETURN_IF(result(&p.out[0], y, rows, out));
-  p.add = static_cast<const __nv_bfloat16*>(add);
-  p.m = rows; p.n = out;
-  p.m_tiles = tiles_of(rows, gemm::kTileM); p.n_tiles = tiles_of(out, bn);
-  p.chunks = p.source_chunks = tiles_of(mid, gemm::kChunk);
-  return launch_any<false, false, gemm::kPlain>(bn, p, stream);
+  p.out[0] = words(y);
+  p.read[0] = words(add);
+  p.m = int(rows); p.n = out;
+  p.source_chunks = q.chunks;
+  return add != nullptr ? launch_plan<false, false, gemm::kPlus>(q, p, nullptr, 0, stream)
+                        : launch_plan<false, false, gemm::kPlain>(q, p, nullptr, 0, stream);
 }
 
-extern "C" int tgt_gated_hidden_grad(const void* dy, const void* w_down, const void* gate, const void* up, int64_t rows, int out,
-                                     int mid, int act, int dtype, void* dgate, void* dup, void* stream_) {
+extern "C" int tgt_gated_hidden_grad(const void* dy, const void* w_down, const void* gate, const void* up, const void* low,
+                                     int64_t rows, int out, int mid, int act, int dtype, void* dgate, void* dup, void* stream_) {
   using namespace tgt;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   TGT_RETURN_IF(check_widths(rows, out, mid, dtype, act));
   if (rows == 0) return TGT_OK;
-  TGT_CHECK_ARG(dy && w_down && gate && up && dgate && dup, "dy, w_down, gate, up, dgate and dup must not be null");
-  TGT_CHECK_ARG(aligned16(dy) && aligned16(w_down) && aligned16(gate) && aligned16(up) && aligned16(dgate) && aligned16(dup),
+  TGT_CHECK_ARG(dy && w_down && gate && up && (low || dtype == TGT_F32) && dgate && dup,
+                "dy, w_down, gate, up, low, dgate and dup must not be null");
+  TGT_CHECK_ARG(aligned16(dy) && aligned16(w_down) && aligned16(gate) && aligned16(up) && aligned16(low) && aligned16(dgate) &&
+                    aligned16(dup),
                 "tensors must be 16-byte aligned");
   if (dtype == TGT_F32) {
     TGT_RETURN_IF(tgt_linear_input_grad(static_cast<const float*>(dy), static_cast<const float*>(w_down), rows, out, mid,
@@ -269,18 +335,17 @@ extern "C" int tgt_gated_hidden_grad(const void* dy, const void* w_down, const v
   }
   Gemm p{};
   TGT_RETURN_IF(expired_wait_word(&p.expired));
-  const int bn = tile_columns_for(rows, mid, 64);
+  const Plan q = plan_for(1, rows, mid, 64, tiles_of(out, gemm::kChunk), kGradTime, false);
   TGT_RETURN_IF(operand(&p.a[0], dy, rows, out, false, gemm::kTileM));
-  TGT_RETURN_IF(operand(&p.b[0], w_down, out, mid, true, bn));
+  TGT_RETURN_IF(operand(&p.b[0], w_down, out, mid, true, q.cut.b_rows()));
   p.a[1] = p.a[0]; p.b[1] = p.b[0];
-  TGT_RETURN_IF(result(&p.out[0], dgate, rows, mid));
-  TGT_RETURN_IF(result(&p.out[1], dup, rows, mid));
-  p.gate = static_cast<const __nv_bfloat16*>(gate); p.up = static_cast<const __nv_bfloat16*>(up);
-  p.m = rows; p.n = mid;
-  p.m_tiles = tiles_of(rows, gemm::kTileM); p.n_tiles = tiles_of(mid, bn);
-  p.chunks = p.source_chunks = tiles_of(out, gemm::kChunk);
+  p.out[0] = words(dgate);
+  p.out[1] = words(dup);
+  p.read[0] = words(gate); p.read[1] = words(up); p.read[2] = words(low);
+  p.m = int(rows); p.n = mid;
+  p.source_chunks = q.chunks;
   p.act = act;
-  return launch_any<false, true, gemm::kGatedGrad>(bn, p, stream);
+  return launch_plan<false, true, gemm::kGatedGrad>(q, p, nullptr, 0, stream);
 }
 
 extern "C" int tgt_gated_input_grad(const void* dgate, const void* dup, const void* w_gate, const void* w_up, int64_t rows, int mid,
@@ -299,17 +364,15 @@ extern "C" int tgt_gated_input_grad(const void* dgate, const void* dup, const vo
   }
   Gemm p{};
   TGT_RETURN_IF(expired_wait_word(&p.expired));
-  const int bn = tile_columns_for(rows, in, 64);
+  const Plan q = plan_for(1, rows, in, 64, 2 * tiles_of(mid, gemm::kChunk), kPlainTime, false);
   TGT_RETURN_IF(operand(&p.a[0], dgate, rows, mid, false, gemm::kTileM));
   TGT_RETURN_IF(operand(&p.a[1], dup, rows, mid, false, gemm::kTileM));
-  TGT_RETURN_IF(operand(&p.b[0], w_gate, mid, in, true, bn));
-  TGT_RETURN_IF(operand(&p.b[1], w_up, mid, in, true, bn));
-  TGT_RETURN_IF(result(&p.out[0], dx, rows, in));
-  p.m = rows; p.n = in;
-  p.m_tiles = tiles_of(rows, gemm::kTileM); p.n_tiles = tiles_of(in, bn);
-  p.source_chunks = tiles_of(mid, gemm::kChunk);
-  p.chunks = 2 * p.source_chunks;
-  return launch_any<false, true, gemm::kPlain>(bn, p, stream);
+  TGT_RETURN_IF(operand(&p.b[0], w_gate, mid, in, true, q.cut.b_rows()));
+  TGT_RETURN_IF(operand(&p.b[1], w_up, mid, in, true, q.cut.b_rows()));
+  p.out[0] = words(dx);
+  p.m = int(rows); p.n = in;
+  p.source_chunks = q.chunks / 2;
+  return launch_plan<false, true, gemm::kPlain>(q, p, nullptr, 0, stream);
 }
 
 extern "C" int tgt_gated_weight_grad_scratch_bytes(int count, int64_t rows, int out_features, int in_features, int dtype,
@@ -319,7 +382,7 @@ extern "C" int tgt_gated_weight_grad_scratch_bytes(int count, int64_t rows, int 
   TGT_CHECK_ARG(count == 1 || count == 2, "count must be 1 or 2");
   TGT_RETURN_IF(check_widths(rows, out_features, in_features, dtype, TGT_ACT_SILU));
   if (dtype == TGT_F32) return tgt_linear_wgrad_multi_scratch_bytes(count, rows, in_features, out_features, bytes);
-  *bytes = rows == 0 ? 0 : plan_parts(count, rows, out_features, in_features).bytes();
+  *bytes = rows == 0 ? 0 : weight_grad_plan(count, rows, out_features, in_features).scratch();
   return TGT_OK;
 }
 
@@ -347,32 +410,15 @@ extern "C" int tgt_gated_weight_grad(const void* const* dy, const void* x, int c
     return tgt_linear_wgrad_multi(d, static_cast<const float*>(x), count, rows, in_features, out_features, w, bias, scratch,
                                   scratch_bytes, stream);
   }
-  const PartsPlan q = plan_parts(count, rows, out_features, in_features);
-  if (scratch == nullptr || scratch_bytes < q.bytes())
-    return set_error(TGT_ERR_WORKSPACE, "scratch holds %zu bytes, %zu needed", scratch_bytes, q.bytes());
+  const Plan q = weight_grad_plan(count, rows, out_features, in_features);
   Gemm p{};
   TGT_RETURN_IF(expired_wait_word(&p.expired));
   for (int i = 0; i < 2; ++i)
     TGT_RETURN_IF(operand(&p.a[i], dy[i < count ? i : 0], rows, out_features, true, gemm::kTileM));
-  TGT_RETURN_IF(operand(&p.b[0], x, rows, in_features, true, q.bn));
+  TGT_RETURN_IF(operand(&p.b[0], x, rows, in_features, true, q.cut.b_rows()));
   p.b[1] = p.b[0];
-  p.partial = static_cast<float*>(scratch);
+  p.out[0] = words(dw[0]); p.out[1] = words(dw[count - 1]);
   p.m = out_features; p.n = in_features;
-  p.m_tiles = q.m_tiles; p.n_tiles = q.n_tiles; p.product_tiles = q.product_tiles;
-  p.chunks = p.source_chunks = q.chunks;
-  gemm::SumParts s{p.partial, {static_cast<__nv_bfloat16*>(dw[0]), static_cast<__nv_bfloat16*>(dw[count - 1])}, out_features,
-                   in_features, q.m_tiles, q.n_tiles, q.product_tiles, q.chunks, q.ctas};
-  const dim3 grid(unsigned(q.m_tiles) * q.n_tiles, 4 * q.bn / 64);
-  if (q.bn == 256) {
-    TGT_RETURN_IF((launch<256, true, true, gemm::kPartial>(p, q.ctas, stream)));
-    gemm::sum_parts_kernel<256><<<grid, gemm::kSumThreads, 0, stream>>>(s);
-  } else if (q.bn == 128) {
-    TGT_RETURN_IF((launch<128, true, true, gemm::kPartial>(p, q.ctas, stream)));
-    gemm::sum_parts_kernel<128><<<grid, gemm::kSumThreads, 0, stream>>>(s);
-  } else {
-    TGT_RETURN_IF((launch<64, true, true, gemm::kPartial>(p, q.ctas, stream)));
-    gemm::sum_parts_kernel<64><<<grid, gemm::kSumThreads, 0, stream>>>(s);
-  }
-  TGT_CHECK_CUDA(cudaGetLastError());
-  return TGT_OK;
+  p.source_chunks = q.chunks;
+  return launch_plan<true, true, gemm::kPlain>(q, p, scratch, scratch_bytes, stream);
 }

@@ -23,7 +23,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     ``w_down`` [out, mid], ``residual`` [..., out] and ``activation`` "silu", "gelu" (exact) or "relu".
 
     In bf16 the activation and its product with the up projection are taken from fp32 sums, as is the residual's addition;
-    what the gradients need of the two projections is kept in bf16."""
+    what the gradients need of the two projections is kept
+    with 16 bits of their sums (6 bytes for a pair)."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}; got {activation!r}")
     if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.dim() != 2 or w_down.shape[1] != w_gate.shape[0] or \
