@@ -631,6 +631,12 @@ TGT_API int tgt_gated_weight_grad(const void* const* dy, const void* x, int coun
                                   int in_features, int dtype, void* const* dw, void* scratch, size_t scratch_bytes,
                                   void* stream);
 
+/*
+ * The block without its gradients for at most 32 rows in bf16 (serving): h [rows, mid] is scratch.  Widths and alignment as above.
+ */
+TGT_API int tgt_gated_few_rows(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* add,
+                               int64_t rows, int in, int mid, int out, int act, void* h, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

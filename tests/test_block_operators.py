@@ -115,3 +115,6 @@ def test_gated_block_arguments():
     assert lib.tgt_gated_weight_grad_scratch_bytes(2, 0, 64, 64, 1, ctypes.byref(n)) == 0 and n.value == 0
     dw = (ctypes.c_void_p * 2)(16, 16)
     assert lib.tgt_gated_weight_grad(None, None, 2, 1, 64, 64, 1, dw, None, 0, None) == 1
+    few = lambda rows, i, m, o, act: lib.tgt_gated_few_rows(None, None, None, None, None, rows, i, m, o, act, None, None, None)  # noqa: E731
+    assert few(0, 64, 64, 64, 3) == 0 and few(1, 64, 64, 64, 3) == 1 and few(33, 64, 64, 64, 3) == 1 and few(-1, 64, 64, 64, 3) == 1
+    assert few(1, 64, 60, 64, 3) == 3 and few(1, 64, 64, 65544, 3) == 3 and few(1, 64, 64, 64, 0) == 1

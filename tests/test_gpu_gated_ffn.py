@@ -105,6 +105,22 @@ def test_bf16(rows, n_in, n_mid, n_out):
     _check(rows, n_in, n_mid, n_out, torch.bfloat16, "silu", rows % 2 == 1)
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 24, 31, 32])
+def test_a_few_rows_without_gradients(rows, act):
+    """As serving calls it: widths around the kernels' steps of 8, 16, 32 and whole turns of k."""
+    from torchgt_b200 import gated_feed_forward
+    for n_in, n_mid, n_out in ((8, 8, 8), (40, 24, 56), (256, 136, 264), (2048, 512, 40), (2056, 4104, 72)):
+        x, wg, wu, wd, r, _ = _inputs(rows, n_in, n_mid, n_out, torch.bfloat16, 23)
+        for residual in (None, r):
+            got = gated_feed_forward(x, wg, wu, wd, act, residual)
+            _within(got, _formula(x, wg, wu, wd, act, residual, None)["y"], (n_in, n_mid, n_out))
+        again = gated_feed_forward(x, wg, wu, wd, act, r)
+        assert torch.equal(again, got)
+        # a row's result does not depend on how many there are beside it
+        assert torch.equal(gated_feed_forward(x[:1], wg, wu, wd, act, r[:1]), got[:1]) or rows > 8
+
+
 @pytest.mark.parametrize("rows,n_in,n_mid,n_out", [(1, 64, 64, 64), (3, 64, 128, 4), (200, 128, 64, 100), (4097, 64, 128, 64), (9000, 64, 64, 64),
                                                    (700, 1024, 1024, 1024)])
 def test_fp32(rows, n_in, n_mid, n_out):

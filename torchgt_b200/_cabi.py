@@ -164,6 +164,8 @@ SIGNATURES = {
     "tgt_gated_weight_grad_scratch_bytes": (c_int, [c_int, c_int64, c_int, c_int, c_int, POINTER(c_size_t)]),
     "tgt_gated_weight_grad": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_size_t,
                                       c_void_p]),
+    "tgt_gated_few_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p,
+                                   c_void_p, c_void_p]),
     "tgt_p2p_control_bytes": (c_size_t, []),
     "tgt_p2p_push": (c_int, [c_void_p, c_void_p, c_void_p, c_int, POINTER(c_void_p), c_size_t, c_int64, c_int64,
                              c_int64, c_int, c_int, c_void_p, c_int, c_int64, c_int, c_void_p]),

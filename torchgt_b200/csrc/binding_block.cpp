@@ -226,6 +226,11 @@ at::Tensor kernel_ready(const at::Tensor& t) {
   return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0 ? c : c.clone();
 }
 
+// Rows without gradients for which the kernels of gated_rows.cu are ahead of tiles of 128 rows.  us, weights not in the L2: 2,048 x
+// 5,632, one row 18 / 46, 16 rows 23 / 43, 32 rows 32 / 37; 768 x 2,048, 32 rows 10 / 19; 4,096 x 11,008, one row 51 / 102, 16 rows
+// 69 / 80, and at 32 rows tiles.
+bool few_rows(int64_t rows, int64_t in, int64_t mid) { return rows <= 16 || (rows <= 32 && in * mid <= int64_t(1) << 24); }
+
 struct GatedFeedForwardBackward : public torch::autograd::Node {
   SavedVariable x, w_gate, w_up, w_down, hidden, gate, up, low;   // low: of bf16 (tgt_gated_hidden)
   int act = TGT_ACT_SILU;
@@ -347,6 +352,11 @@ at::Tensor gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const a
     sizes.back() = out;
     y = at::empty(sizes, x.options());
     void* const stream = stream_of(x);
+    if (type == TGT_BF16 && !record && few_rows(rows, in, mid)) {
+      check(tgt_gated_few_rows(ptr(xc), ptr(wgc), ptr(wuc), ptr(wdc), ptr(rc), rows, int(in), int(mid), int(out), act, ptr(h), ptr(y),
+                               stream));
+      return y;
+    }
     check(tgt_gated_hidden(ptr(xc), ptr(wgc), ptr(wuc), rows, int(in), int(mid), act, type, ptr(h), ptr(g), ptr(u), ptr(l), stream));
     check(tgt_gated_output(ptr(h), ptr(wdc), ptr(rc), rows, int(mid), int(out), type, ptr(y), stream));
   }
