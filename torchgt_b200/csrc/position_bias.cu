@@ -36,7 +36,7 @@ struct BiasFwd {
 
 template <typename Id, typename Pos>
 __device__ __forceinline__ int bucket_of(const BiasFwd& p, const int32_t* borders, int64_t e) {
-  int64_t s = static_cast<const Id*>(p.source)[e], d = static_cast<const Id*>(p.destination)[e];
+  int64_t s = __ldcs(static_cast<const Id*>(p.source) + e), d = __ldcs(static_cast<const Id*>(p.destination) + e);
   if (p.positions != nullptr) {
     if (s < 0 || s >= p.n_positions || d < 0 || d >= p.n_positions) return kNoBucket;
     s = __ldg(static_cast<const Pos*>(p.positions) + s);
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kBiasThreads) position_bias_kernel(const __gri
       if constexpr (VEC == 4) {
         float4 v = make_float4(nan, nan, nan, nan);
         if (b != kNoBucket) v = __ldg(reinterpret_cast<const float4*>(p.table) + b * pieces + (piece - of * pieces));
-        reinterpret_cast<float4*>(out)[piece] = v;
+        __stcs(reinterpret_cast<float4*>(out) + piece, v);
       } else {
         out[piece] = b != kNoBucket ? __ldg(p.table + b * pieces + (piece - of * pieces)) : nan;
       }
@@ -92,6 +92,12 @@ struct BiasBwd {
   int n_buckets, heads;
 };
 
+struct TableSum {
+  const float* partial;        // [ctas][values]
+  float* dtable;
+  int ctas, values;
+};
+
 // HP: heads of a warp, a power of two; blockIdx.y picks which
 template <int HP>
 __global__ void __launch_bounds__(kBiasThreads) position_bias_grad_kernel(const BiasBwd p) {
@@ -102,24 +108,42 @@ __global__ void __launch_bounds__(kBiasThreads) position_bias_grad_kernel(const 
   constexpr int kSlots = 32 / HP;                            // edges of a group
   const int slot = lane / HP, h0 = blockIdx.y * 32, h = h0 + lane % HP;
   const bool has_head = h < p.heads;
-  constexpr int kBatch = HP < 8 ? HP : 8;                    // rows in flight
-  for (int64_t e0 = (int64_t(blockIdx.x) * warps + warp) * 32; e0 < p.n_edges; e0 += int64_t(gridDim.x) * warps * 32) {
-    const int bucket = e0 + lane < p.n_edges ? p.buckets[e0 + lane] : kNoBucket;
+  // A batch is eight groups; the next one's rows are on their way while this one's are added, whose sums in shared memory wait
+  // for one another (as far as the compiler can know).
+  constexpr int kBatch = 8, kEdges = kBatch * kSlots, kWords = kEdges > 32 ? kEdges / 32 : 1;
+  const int64_t step = int64_t(gridDim.x) * warps * kEdges;
+  int64_t e0 = (int64_t(blockIdx.x) * warps + warp) * kEdges;
+  float next[kBatch];
+  int next_bucket[kWords];
+  auto load = [&]() {
 #pragma unroll
-    for (int i0 = 0; i0 < HP; i0 += kBatch) {
-      float v[kBatch];
+    for (int k = 0; k < kWords; ++k) {
+      const int64_t e = e0 + 32 * k + lane;
+      next_bucket[k] = e < p.n_edges && 32 * k + lane < kEdges ? __ldcs(p.buckets + e) : kNoBucket;
+    }
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int64_t e = e0 + (i0 + i) * kSlots + slot;
-        v[i] = has_head && e < p.n_edges ? __ldg(p.dbias + e * p.heads + h) : 0.f;
-      }
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t e = e0 + i * kSlots + slot;
+      next[i] = has_head && e < p.n_edges ? __ldcs(p.dbias + e * p.heads + h) : 0.f;
+    }
+  };
+  load();
+  while (e0 < p.n_edges) {
+    float v[kBatch];
+    int bucket[kWords];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int b = __shfl_sync(0xffffffffu, bucket, (i0 + i) * kSlots + slot);
-        if (b != kNoBucket) sums[b * 32 + lane] += v[i];
-      }
+    for (int i = 0; i < kBatch; ++i) v[i] = next[i];
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) bucket[k] = next_bucket[k];
+    e0 += step;
+    load();
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int b = __shfl_sync(0xffffffffu, bucket[i * kSlots / 32], i * kSlots % 32 + slot);
+      if (b != kNoBucket) sums[b * 32 + lane] += v[i];
     }
   }
+  release_dependents();
   __syncthreads();
   for (int i = threadIdx.x; i < p.n_buckets * HP; i += blockDim.x) {
     const int b = i / HP, head = i % HP;
@@ -132,12 +156,26 @@ __global__ void __launch_bounds__(kBiasThreads) position_bias_grad_kernel(const 
   }
 }
 
-__global__ void __launch_bounds__(kPartialSumThreads) position_bias_table_kernel(const float* partial, int n_parts, int values,
-                                                                                 float* dtable) {
-  __shared__ float s_part[16][32];
-  const int i = blockIdx.x * 32 + threadIdx.x % 32;
-  const float s = sum_partials(partial, n_parts, values, i, i < values, s_part);
-  if (threadIdx.x < 32 && i < values) dtable[i] = s;
+// A block adds 32 values of the CTAs' sums: 32 warps, eight in flight each.
+constexpr int kTableThreads = 1024;
+__global__ void __launch_bounds__(kTableThreads) position_bias_table_kernel(const TableSum p) {
+  __shared__ float s_part[32][33];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, i = blockIdx.x * 32 + lane;
+  float s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = 0.f;
+  dependent_wait();
+  if (i < p.values)
+    for (int c = warp; c < p.ctas; c += 32 * 8)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + 32 * j < p.ctas) s[j] += __ldcg(p.partial + int64_t(c + 32 * j) * p.values + i);
+  s_part[warp][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+  __syncthreads();
+  float v = s_part[lane][warp];                   // of value `warp` of the block, the sums of warp `lane`
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lane == 0 && blockIdx.x * 32 + warp < p.values) p.dtable[blockIdx.x * 32 + warp] = v;
 }
 
 struct GradPlan {
@@ -155,7 +193,7 @@ GradPlan plan_grad(int64_t n_edges, int n_buckets, int heads) {
   int resident = kMostSmem / g.smem;
   resident = resident > 6 ? 6 : resident;
   // a CTA clears and adds up its sums: at least eight steps a warp before there is a second
-  const int64_t steps = (n_edges + 31) / 32, want = (steps + 8 * g.warps - 1) / (8 * g.warps);
+  const int64_t batch = 8 * (32 / g.hp), steps = (n_edges + batch - 1) / batch, want = (steps + 8 * g.warps - 1) / (8 * g.warps);
   const int64_t most = int64_t(sm_count()) * resident;
   g.ctas = int(want < 1 ? 1 : want > most ? most : want);
   return g;
@@ -166,6 +204,7 @@ int launch_grad(const BiasBwd& p, const GradPlan& g, cudaStream_t stream) {
   const int rc = allow_shared_memory<position_bias_grad_kernel<HP>>(kMostSmem);
   if (rc != TGT_OK) return rc;
   position_bias_grad_kernel<HP><<<dim3(g.ctas, (p.heads + 31) / 32), g.warps * 32, g.smem, stream>>>(p);
+  TGT_CHECK_CUDA(cudaGetLastError());
   return TGT_OK;
 }
 
@@ -262,7 +301,7 @@ extern "C" int tgt_edge_position_bias_grad(const float* dbias, const uint16_t* b
     default: rc = launch_grad<32>(p, g, stream); break;
   }
   if (rc != TGT_OK) return rc;
-  position_bias_table_kernel<<<(values + 31) / 32, kPartialSumThreads, 0, stream>>>(p.partial, g.ctas, values, dtable);
-  TGT_CHECK_CUDA(cudaGetLastError());
+  const TableSum sum{p.partial, dtable, g.ctas, values};
+  TGT_CHECK_CUDA(launch_chained(position_bias_table_kernel, dim3((values + 31) / 32), kTableThreads, stream, kLinkStitch, sum));
   return TGT_OK;
 }

@@ -70,13 +70,16 @@ struct LargestBits {   // of non-negative values as whole numbers: NaN is above 
     return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
   }
 };
+// `turn` changes with every sum: a sum's words are not written again before all have passed the barrier of the next.
+constexpr int kPartWords = 64;
 template <int LPR, class Op>
-__device__ __forceinline__ float over_row(float x, float* s_part, Op op) {
+__device__ __forceinline__ float over_row(float x, float* s_part, int& turn, Op op) {
 #pragma unroll
   for (int o = (LPR == 0 ? 32 : LPR) / 2; o > 0; o >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, o));
   if constexpr (LPR == 0) {
     const int warps = blockDim.x / 32;
-    __syncthreads();                              // the sums before this one have been read
+    s_part += turn;
+    turn ^= 32;
     if (threadIdx.x % 32 == 0) s_part[threadIdx.x / 32] = x;
     __syncthreads();
     x = s_part[0];
@@ -100,6 +103,8 @@ struct Place {
     step = LPR == 0 ? blockDim.x : LPR;
   }
 };
+// Whether a thread has registers for the next row while it works on one: 32-bit words of a matrix that it holds
+constexpr bool row_ahead(int pieces, int vec, size_t value, int most) { return pieces * (vec == 1 ? 1 : int(vec * value / 4)) <= most; }
 constexpr int most_threads(int lpr, int vec) { return lpr != 0 ? kGroupThreads : vec == 1 ? 1024 : 512; }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
@@ -120,24 +125,37 @@ struct RmsFwd {
 
 template <typename T, int VEC, int LPR, int PIECES, bool E4M3>
 __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_fwd_kernel(const RmsFwd<T> p) {
-  __shared__ float s_part[32];
+  __shared__ float s_part[kPartWords];
+  int turn = 0;
   const Place<LPR> at;
   const int pieces = p.hidden / VEC;
   const float inv_hidden = 1.f / float(p.hidden);
+  Piece<T, VEC> next[PIECES], next_res[PIECES];              // the next row, on its way
+  auto load = [&](int64_t r) {
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int c = at.first + j * at.step;
+      if (r < p.rows && c < pieces) {
+        next[j].load(p.x + r * p.hidden, c);
+        if (p.residual != nullptr) next_res[j].load(p.residual + r * p.hidden, c);
+      } else {
+        next[j].clear();
+      }
+    }
+  };
+  constexpr bool kAhead = row_ahead(PIECES, VEC, sizeof(T), 16);
+  if (kAhead) load(at.first_row + at.row_of_cta);
   for (int64_t r0 = at.first_row; r0 < p.rows; r0 += at.rows_at_once) {
     const int64_t r = r0 + at.row_of_cta;
     const bool live = r < p.rows;
     Piece<T, VEC> x[PIECES], res[PIECES];
+    if (!kAhead) load(r);
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
-      const int c = at.first + j * at.step;
-      if (live && c < pieces) {
-        x[j].load(p.x + r * p.hidden, c);
-        if (p.residual != nullptr) res[j].load(p.residual + r * p.hidden, c);
-      } else {
-        x[j].clear();
-      }
+      x[j] = next[j];
+      res[j] = next_res[j];
     }
+    if (kAhead) load(r + at.rows_at_once);
     float v[PIECES][VEC], squares = 0.f;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
@@ -153,7 +171,7 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_fwd_kernel(co
 #pragma unroll
       for (int i = 0; i < VEC; ++i) squares = fmaf(v[j][i], v[j][i], squares);
     }
-    squares = over_row<LPR>(squares, s_part, Add());
+    squares = over_row<LPR>(squares, s_part, turn, Add());
     const float rstd = rsqrtf(squares * inv_hidden + p.eps);
     if (live && at.first == 0 && p.rstd != nullptr) p.rstd[r] = rstd;
     float largest = 0.f;
@@ -173,7 +191,7 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_fwd_kernel(co
       if (!E4M3) Piece<T, VEC>::store(p.y + r * p.hidden, c, v[j]);
     }
     if constexpr (E4M3) {
-      largest = over_row<LPR>(largest, s_part, LargestBits());
+      largest = over_row<LPR>(largest, s_part, turn, LargestBits());
       float scale = largest / 448.f;
       scale = scale < 0x1p-126f ? 0x1p-126f : scale;          // NaN stays
       const float by = 1.f / scale;
@@ -206,7 +224,8 @@ struct RmsBwd {
 
 template <typename T, int VEC, int LPR, int PIECES>
 __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_bwd_kernel(const RmsBwd<T> p) {
-  __shared__ float s_part[32];
+  __shared__ float s_part[kPartWords];
+  int turn = 0;
   extern __shared__ float s_dw[];               // [warps][hidden], where rows belong to groups of lanes
   const Place<LPR> at;
   const int pieces = p.hidden / VEC;
@@ -221,23 +240,38 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_bwd_kernel(co
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[j][i] = 0.f;
   }
+  Piece<T, VEC> next[PIECES], next_dy[PIECES], next_ds[PIECES];   // the next row, on its way
+  float next_rstd;
+  auto load = [&](int64_t r) {
+    next_rstd = r < p.rows ? __ldg(p.rstd + r) : 0.f;
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int c = at.first + j * at.step;
+      if (r < p.rows && c < pieces) {
+        next[j].load(p.v + r * p.hidden, c);
+        next_dy[j].load(p.dy + r * p.hidden, c);
+        if (p.dsum != nullptr) next_ds[j].load(p.dsum + r * p.hidden, c);
+      } else {
+        next[j].clear();
+        next_dy[j].clear();
+      }
+    }
+  };
+  constexpr bool kAhead = LPR == 0 && row_ahead(PIECES, VEC, sizeof(T), 8);
+  if (kAhead) load(at.first_row + at.row_of_cta);
   for (int64_t r0 = at.first_row; r0 < p.rows; r0 += at.rows_at_once) {
     const int64_t r = r0 + at.row_of_cta;
     const bool live = r < p.rows;
     Piece<T, VEC> v[PIECES], dy[PIECES], ds[PIECES];
-    const float rstd = live ? __ldg(p.rstd + r) : 0.f;
+    if (!kAhead) load(r);
+    const float rstd = next_rstd;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
-      const int c = at.first + j * at.step;
-      if (live && c < pieces) {
-        v[j].load(p.v + r * p.hidden, c);
-        dy[j].load(p.dy + r * p.hidden, c);
-        if (p.dsum != nullptr) ds[j].load(p.dsum + r * p.hidden, c);
-      } else {
-        v[j].clear();
-        dy[j].clear();
-      }
+      v[j] = next[j];
+      dy[j] = next_dy[j];
+      ds[j] = next_ds[j];
     }
+    if (kAhead) load(r + at.rows_at_once);
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
@@ -252,7 +286,7 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_bwd_kernel(co
         dot = fmaf(d[i] * g[i], u, dot);
       }
     }
-    dot = over_row<LPR>(dot, s_part, Add()) * inv_hidden;
+    dot = over_row<LPR>(dot, s_part, turn, Add()) * inv_hidden;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
       const int c = at.first + j * at.step;
@@ -271,6 +305,7 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_bwd_kernel(co
       Piece<T, VEC>::store(p.dx + r * p.hidden, c, d);
     }
   }
+  release_dependents();
   float* out = p.partial + int64_t(blockIdx.x) * p.hidden;
   if constexpr (LPR == 0) {
 #pragma unroll
@@ -302,12 +337,32 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_bwd_kernel(co
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kPartialSumThreads) rms_norm_weight_grad_kernel(const float* partial, int n_parts, int hidden,
-                                                                                  T* dweight) {
-  __shared__ float s_part[16][32];
-  const int i = blockIdx.x * 32 + threadIdx.x % 32;
-  const float s = sum_partials(partial, n_parts, hidden, i, i < hidden, s_part);
-  if (threadIdx.x < 32 && i < hidden) dweight[i] = T(s);
+struct WeightSum {
+  const float* partial;        // [parts][hidden]
+  T* dweight;
+  int parts, hidden;
+};
+// A block adds 32 values of the CTAs' sums: 32 warps, eight in flight each.
+constexpr int kSumThreads = 1024;
+template <typename T>
+__global__ void __launch_bounds__(kSumThreads) rms_norm_weight_grad_kernel(const WeightSum<T> p) {
+  __shared__ float s_sum[32][33];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, i = blockIdx.x * 32 + lane;
+  float s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = 0.f;
+  dependent_wait();
+  if (i < p.hidden)
+    for (int c = warp; c < p.parts; c += 32 * 8)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + 32 * j < p.parts) s[j] += __ldcg(p.partial + int64_t(c + 32 * j) * p.hidden + i);
+  s_sum[warp][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+  __syncthreads();
+  float v = s_sum[lane][warp];                   // of value `warp` of the block, the sums of warp `lane`
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lane == 0 && blockIdx.x * 32 + warp < p.hidden) p.dweight[blockIdx.x * 32 + warp] = T(v);
 }
 
 // ---- which kernel ----------------------------------------------------------------------------------------------------
@@ -407,9 +462,9 @@ int launch_backward(RmsBwd<T> p, void* dweight, void* scratch, size_t scratch_by
       rms_norm_bwd_kernel<T, VEC, kLpr, kPieces><<<grid, s.threads, smem, stream>>>(p);
   });
   if (!built) return set_error(TGT_ERR_UNSUPPORTED, "no kernel for hidden=%d", p.hidden);
-  rms_norm_weight_grad_kernel<T><<<(p.hidden + 31) / 32, kPartialSumThreads, 0, stream>>>(p.partial, grid, p.hidden,
-                                                                                        static_cast<T*>(dweight));
   TGT_CHECK_CUDA(cudaGetLastError());
+  const WeightSum<T> sum{p.partial, static_cast<T*>(dweight), grid, p.hidden};
+  TGT_CHECK_CUDA(launch_chained(rms_norm_weight_grad_kernel<T>, dim3((p.hidden + 31) / 32), kSumThreads, stream, kLinkStitch, sum));
   return TGT_OK;
 }
 
