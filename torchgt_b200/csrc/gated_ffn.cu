@@ -5,7 +5,8 @@
 // bf16: five products of gated_gemm.cuh.  The gate's and the up projection's columns of a tile are summed side by side, so
 // the activation and their product are taken from fp32 sums before anything is rounded; dg and du leave the product that makes dh,
 // dx is one sum over both, and each weight's gradient is summed over rows that all SMs share.
-// fp32: the split products of linear_mma.cu, with the gate between them in kernels of their own.
+// fp32: the split products of linear_mma.cu with the gate in their finish, or, for reductions over several launches and few rows,
+// with the gate in kernels of its own.
 #include <atomic>
 
 #include "gated_gemm.cuh"
@@ -202,39 +203,23 @@ int check_widths(int64_t rows, int a, int b, int dtype, int act) {
 
 // ---- fp32: the gate between the products -------------------------------------------------------------------------------
 constexpr int kGateThreads = 256;
-template <bool SLOPE>
-__device__ __forceinline__ float act_f32(int act, float x, float& slope) {
-  if (act == TGT_ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-x));
-    if (SLOPE) slope = s * (1.f + x * (1.f - s));
-    return x * s;
-  }
-  if (act == TGT_ACT_GELU) {
-    if (SLOPE) slope = gelu_slope(x);
-    return gelu(x);
-  }
-  if (SLOPE) slope = x <= 0.f ? 0.f : 1.f;
-  return relu(x);
-}
 __global__ void __launch_bounds__(kGateThreads) gate_kernel(const float4* gate, const float4* up, int64_t n, int act, float4* h) {
-  for (int64_t i = blockIdx.x * int64_t(kGateThreads) + threadIdx.x; i < n; i += int64_t(gridDim.x) * kGateThreads) {
-    const float4 g = __ldg(gate + i), u = __ldg(up + i);
-    float unused;
-    h[i] = make_float4(act_f32<false>(act, g.x, unused) * u.x, act_f32<false>(act, g.y, unused) * u.y,
-                       act_f32<false>(act, g.z, unused) * u.z, act_f32<false>(act, g.w, unused) * u.w);
-  }
+  with_activation(act, [&](auto a) {
+    for (int64_t i = blockIdx.x * int64_t(kGateThreads) + threadIdx.x; i < n; i += int64_t(gridDim.x) * kGateThreads)
+      h[i] = gated<decltype(a)::value>(__ldg(gate + i), __ldg(up + i));
+  });
 }
 // dgate holds dh and receives dgate
 __global__ void __launch_bounds__(kGateThreads) gate_grad_kernel(const float4* gate, const float4* up, int64_t n, int act,
                                                                  float4* dgate, float4* dup) {
-  for (int64_t i = blockIdx.x * int64_t(kGateThreads) + threadIdx.x; i < n; i += int64_t(gridDim.x) * kGateThreads) {
-    const float4 g = __ldg(gate + i), u = __ldg(up + i), d = dgate[i];
-    float4 slope, a;
-    a.x = act_f32<true>(act, g.x, slope.x); a.y = act_f32<true>(act, g.y, slope.y);
-    a.z = act_f32<true>(act, g.z, slope.z); a.w = act_f32<true>(act, g.w, slope.w);
-    dgate[i] = make_float4(d.x * u.x * slope.x, d.y * u.y * slope.y, d.z * u.z * slope.z, d.w * u.w * slope.w);
-    dup[i] = make_float4(d.x * a.x, d.y * a.y, d.z * a.z, d.w * a.w);
-  }
+  with_activation(act, [&](auto a) {
+    for (int64_t i = blockIdx.x * int64_t(kGateThreads) + threadIdx.x; i < n; i += int64_t(gridDim.x) * kGateThreads) {
+      float4 dg, du;
+      gated_grad<decltype(a)::value>(dgate[i], __ldg(gate + i), __ldg(up + i), dg, du);
+      dgate[i] = dg;
+      dup[i] = du;
+    }
+  });
 }
 int gate_grid(int64_t n) {
   const int64_t want = (n + kGateThreads - 1) / kGateThreads, most = int64_t(sm_count()) * 8;
@@ -258,9 +243,13 @@ extern "C" int tgt_gated_hidden(const void* x, const void* w_gate, const void* w
                 "tensors must be 16-byte aligned");
   if (dtype == TGT_F32) {
     TGT_CHECK_ARG(gate != nullptr, "in fp32 gate and up must not be null");
+    if (in > 1024 || mid > 1024 || in % 4 != 0 || mid % 4 != 0)
+      return set_error(TGT_ERR_UNSUPPORTED, "in=%d mid=%d: both must be multiples of 4, at most 1024", in, mid);
     const float* w[2] = {static_cast<const float*>(w_gate), static_cast<const float*>(w_up)};
     const float* bias[2] = {nullptr, nullptr};
     float* c[2] = {static_cast<float*>(gate), static_cast<float*>(up)};
+    if (gated_in_one(rows, in, 2 * mid))
+      return linear_gated(static_cast<const float*>(x), w[0], w[1], rows, in, mid, act, static_cast<float*>(h), c[0], c[1], stream);
     TGT_RETURN_IF(tgt_linear_rows_multi(static_cast<const float*>(x), w, bias, 2, rows, in, mid, TGT_ACT_NONE, nullptr, nullptr, c,
                                         stream));
     const int64_t n = rows * mid / 4;
@@ -325,6 +314,12 @@ extern "C" int tgt_gated_hidden_grad(const void* dy, const void* w_down, const v
                     aligned16(dup),
                 "tensors must be 16-byte aligned");
   if (dtype == TGT_F32) {
+    if (out > 1024 || mid > 1024 || out % 4 != 0 || mid % 4 != 0)
+      return set_error(TGT_ERR_UNSUPPORTED, "out=%d mid=%d: both must be multiples of 4, at most 1024", out, mid);
+    if (gated_in_one(rows, out, mid))
+      return linear_gated_grad(static_cast<const float*>(dy), static_cast<const float*>(w_down), static_cast<const float*>(gate),
+                               static_cast<const float*>(up), rows, out, mid, act, static_cast<float*>(dgate), static_cast<float*>(dup),
+                               stream);
     TGT_RETURN_IF(tgt_linear_input_grad(static_cast<const float*>(dy), static_cast<const float*>(w_down), rows, out, mid,
                                         static_cast<float*>(dgate), stream));
     const int64_t n = rows * mid / 4;

@@ -12,8 +12,6 @@
 // gradients read without a transposed copy).
 #pragma once
 
-#include <type_traits>
-
 #include "linear_rows.cuh"
 #include "tma.cuh"
 
@@ -186,14 +184,6 @@ __device__ __forceinline__ float activate(float x, float& slope) {
     return relu(x);
   }
 }
-// f(the activation as a constant), so that a tile's values branch once
-template <class F>
-__device__ __forceinline__ void with_activation(int act, F&& f) {
-  if (act == TGT_ACT_SILU) f(std::integral_constant<int, TGT_ACT_SILU>());
-  else if (act == TGT_ACT_GELU) f(std::integral_constant<int, TGT_ACT_GELU>());
-  else f(std::integral_constant<int, TGT_ACT_RELU>());
-}
-
 // How the two projections are kept for the gradients: the upper 16 bits of each fp32 sum, and the 8 bits below those of both in
 // a third word.  Their rounding would be in every gradient, next to the roundings of dgate, dup and the result that cannot be avoided: kept in
 // bf16 dx, dWg and dWu are 3.1e-3 from 64 bits (2-norm), with the 8 bits 2.4e-3, rounding the results alone 1.7e-3.

@@ -36,12 +36,17 @@ constexpr int kPieceW = kCols * 128;
 constexpr int kMostSums = 3;               // running sums of large products per tile, of at most two chunks each
 constexpr int kMostChunks = 2 * kMostSums; // of one launch; the weights' pieces of all of them are kept
 
+// What is done with the sums: any of LinearRows' finishes; nothing but a bias; the gated block's two (linear_rows.cuh), where a
+// tile is 32 columns of each projection, 8 and 8 in turn (w[0] and w[1]; c: h, gate, up), or where c is {dgate, dup}.
+enum Finish { kAny, kPlain, kGated, kGatedGrad };
+
 struct SplitGemm : LinearRows {
   int col_tiles;                    // per output
   int first, chunks;                // the part of the reduction this launch sums, in chunks (sources one after the other)
   int big_sums;                     // of two chunks each, the last perhaps of one
   int ahead;                        // tiles between the one whose products run and the one that is brought into the L2, or 0
   int* expired;                     // expired_wait_word
+  const float* up;                  // kGatedGrad, next to gate
 };
 // Tensor memory of a CTA: for each of two tiles the first sum of large products, the sum of small ones, more sums of large ones
 constexpr int tile_columns(bool more) { return (more ? 1 + kMostSums : 2) * kCols; }
@@ -55,10 +60,11 @@ __device__ __forceinline__ int block_offset(int row, int piece) { return row * 6
 // of such rows (bits of `rows`, counted from row0) that are not finite are summed again from the operands themselves, a row at a
 // time by the whole warp: a lane has one of the 16 columns of the warp's block and every other reduction element.  (320,000 rows
 // of 64 x 64, one row not finite: 43 us, with a thread per row and column after column 200; all rows 2.5 ms and 4.9.)
-template <int UNROLL>
+template <int UNROLL, bool GATED>
 __device__ __forceinline__ void sum_rows_again(const SplitGemm& p, int out, int64_t row0, uint32_t rows, int col, uint8_t* block) {
   const int src_chunks = (p.red + kChunk - 1) / kChunk, lane = threadIdx.x % 32;
-  col += lane % 16;
+  if (GATED) out = lane % 16 / 8;                           // eight columns of w[0], the same of w[1]
+  col += GATED ? lane % 8 : lane % 16;
   __syncwarp();                                             // the block is complete
   for (; rows != 0; rows &= rows - 1) {
     const int r = __ffs(rows) - 1;
@@ -80,19 +86,24 @@ __device__ __forceinline__ void sum_rows_again(const SplitGemm& p, int out, int6
 }
 
 // as a call, which costs fewer registers where the finish has need of them itself
+template <bool GATED>
 __device__ __noinline__ void sum_rows_again_called(const SplitGemm& p, int out, int64_t row0, uint32_t rows, int col, uint8_t* block) {
-  sum_rows_again<2>(p, out, row0, rows, col, block);
+  sum_rows_again<2, GATED>(p, out, row0, rows, col, block);
 }
 
 // A wait for the products has run out: this CTA's results from `tile` on become NaN.
+template <Finish FINISH>
 __device__ __noinline__ void give_up(const SplitGemm& p, int out, int c0, int64_t tile, int walkers) {
   if (threadIdx.x == 0) tc::report_expired_wait(p.expired);
   const float nan = __int_as_float(0x7fffffff);
   const int col = c0 + 4 * (threadIdx.x % 16);
-  if (col >= p.cols) return;
+  if (col >= p.cols || (FINISH == kGated && threadIdx.x % 16 >= 8)) return;
+  constexpr int kResults = FINISH == kGated ? 3 : FINISH == kGatedGrad ? 2 : 1;
   for (; tile * kRows < p.rows; tile += walkers)
     for (int64_t row = tile * kRows + threadIdx.x / 16; row < min((tile + 1) * kRows, p.rows); row += kWorkers / 16) {
-      *reinterpret_cast<float4*>(p.c[out] + row * p.cols + col) = make_float4(nan, nan, nan, nan);
+#pragma unroll
+      for (int i = 0; i < kResults; ++i)
+        *reinterpret_cast<float4*>(p.c[kResults > 1 ? i : out] + row * p.cols + col) = make_float4(nan, nan, nan, nan);
       if (p.pre != nullptr) *reinterpret_cast<float4*>(p.pre + row * p.cols + col) = make_float4(nan, nan, nan, nan);
     }
 }
@@ -105,8 +116,9 @@ __host__ __device__ inline int split_gemm_smem(int chunks) {
 static_assert(3 * kPieceA + kMostChunks * 3 * kPieceW + kWarps * kBlockBytes + 16 <= 227 * 1024, "one CTA per SM");
 static_assert(2 * (3 * kPieceA + 2 * 3 * kPieceW + kWarps * kBlockBytes + 16 + 1024) <= 228 * 1024, "two with two chunks");
 
-template <bool PLAIN, bool LONG>   // nothing but a bias is added to the sums; more than two chunks
+template <Finish FINISH, bool LONG>   // LONG: more than two chunks
 __global__ void __launch_bounds__(kThreads, LONG ? 1 : 2) split_gemm_kernel(const __grid_constant__ SplitGemm p) {
+  constexpr bool PLAIN = FINISH == kPlain;
   extern __shared__ __align__(1024) uint8_t s_raw[];
   const int src_chunks = (p.red + kChunk - 1) / kChunk;
   const uint32_t s_a = tc::smem_address(s_raw);
@@ -117,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, LONG ? 1 : 2) split_gemm_kernel(cons
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int across = p.col_tiles * p.outputs;               // neighbours in the grid read the same rows of A
   const int tile_col = blockIdx.x % across;
-  const int out = tile_col / p.col_tiles, c0 = tile_col % p.col_tiles * kCols;
+  const int out = tile_col / p.col_tiles, c0 = tile_col % p.col_tiles * (FINISH == kGated ? kCols / 2 : kCols);
   const int walkers = gridDim.x / across;
   const int64_t tiles = (p.rows + kRows - 1) / kRows;
 
@@ -153,7 +165,12 @@ __global__ void __launch_bounds__(kThreads, LONG ? 1 : 2) split_gemm_kernel(cons
     for (int u = tid; u < kCols * 16; u += kWorkers) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       int n, k;
-      if (!p.transposed) {
+      if constexpr (FINISH == kGated) {
+        n = u / 16; k = 4 * (u % 16);
+        const int col = c0 + n / 16 * 8 + n % 8;
+        if (col < p.cols && k0 + k < p.red)
+          v = __ldg(reinterpret_cast<const float4*>(p.w[n / 8 % 2] + int64_t(col) * p.red + k0 + k));
+      } else if (!p.transposed) {
         n = u / 16; k = 4 * (u % 16);
         if (c0 + n < p.cols && k0 + k < p.red)
           v = __ldg(reinterpret_cast<const float4*>(w + int64_t(c0 + n) * p.red + k0 + k));
@@ -189,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, LONG ? 1 : 2) split_gemm_kernel(cons
       tc::read16(sums + j, big);
       tc::read16(sums + kCols + j, small);
       tc::reads_done();
-      const int col = c0 + warp / 4 * 32 + j;
+      const int col = FINISH == kGated ? c0 + (warp / 4 * 32 + j) / 2 : c0 + warp / 4 * 32 + j;
       float v[16], size = 0.f;
 #pragma unroll
       for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(big[x]) + __uint_as_float(small[x]);
@@ -207,10 +224,59 @@ __global__ void __launch_bounds__(kThreads, LONG ? 1 : 2) split_gemm_kernel(cons
       }
       const uint32_t odd = __ballot_sync(~0u, !(size < __int_as_float(0x7f800000)));
       if (odd != 0) {
-        if (PLAIN) sum_rows_again<4>(p, out, row0, odd, col, s_block);
-        else sum_rows_again_called(p, out, row0, odd, col, s_block);
+        if (PLAIN) sum_rows_again<4, false>(p, out, row0, odd, col, s_block);
+        else sum_rows_again_called<FINISH == kGated>(p, out, row0, odd, col, s_block);
       }
       __syncwarp();
+      if constexpr (FINISH == kGated) {
+        // a lane has four columns of both projections in two rows
+        const int my_col = col + 4 * (lane % 2);
+        with_activation(p.act, [&](auto act) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = lane / 2 + 16 * i;
+            const float4 g = *reinterpret_cast<const float4*>(s_block + block_offset(r, lane % 2));
+            const float4 u = *reinterpret_cast<const float4*>(s_block + block_offset(r, 2 + lane % 2));
+            if (row0 + r >= p.rows || my_col >= p.cols) continue;
+            const int64_t at = (row0 + r) * p.cols + my_col;
+            *reinterpret_cast<float4*>(p.c[1] + at) = g;
+            *reinterpret_cast<float4*>(p.c[2] + at) = u;
+            *reinterpret_cast<float4*>(p.c[0] + at) = gated<decltype(act)::value>(g, u);
+          }
+        });
+        __syncwarp();
+        continue;
+      }
+      if constexpr (FINISH == kGatedGrad) {
+        const int my_col = col + 4 * (lane % 4);
+        with_activation(p.act, [&](auto act) {
+#pragma unroll
+          for (int half = 0; half < 4; half += 2) {      // two rows' operands are on their way together
+            float4 g[2], u[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int64_t row = row0 + lane / 4 + 8 * (half + i);
+              const bool there = row < p.rows && my_col < p.cols;
+              const int64_t at = there ? row * p.cols + my_col : 0;
+              g[i] = __ldg(reinterpret_cast<const float4*>(p.gate + at));
+              u[i] = __ldg(reinterpret_cast<const float4*>(p.up + at));
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int r = lane / 4 + 8 * (half + i);
+              const float4 d = *reinterpret_cast<const float4*>(s_block + block_offset(r, lane % 4));
+              if (row0 + r >= p.rows || my_col >= p.cols) continue;
+              const int64_t at = (row0 + r) * p.cols + my_col;
+              float4 dg, du;
+              gated_grad<decltype(act)::value>(d, g[i], u[i], dg, du);
+              *reinterpret_cast<float4*>(p.c[0] + at) = dg;
+              *reinterpret_cast<float4*>(p.c[1] + at) = du;
+            }
+          }
+        });
+        __syncwarp();
+        continue;
+      }
       const int my_col = col + 4 * (lane % 4);
       if (my_col < p.cols) {
         float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -222,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, LONG ? 1 : 2) split_gemm_kernel(cons
           const int r = lane / 4 + 8 * i;
           const float4 v = *reinterpret_cast<const float4*>(s_block + block_offset(r, lane % 4));
           if (r >= left) continue;
-          if (PLAIN) {
+          if constexpr (PLAIN) {
             *reinterpret_cast<float4*>(c + int64_t(8 * i) * p.cols) = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
           } else {
             finish_values(p, out, row0 + r, my_col, v);
@@ -299,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, LONG ? 1 : 2) split_gemm_kernel(cons
     }
     if (!__syncthreads_and(ok)) failed = before;
   last:
-    if (failed >= 0) give_up(p, out, c0, failed, walkers);
+    if (failed >= 0) give_up<FINISH>(p, out, c0, failed, walkers);
     else if (before >= 0) finish(before, tmem + (sums == tmem ? kHalf : 0));
   }
 finished:
@@ -311,19 +377,20 @@ finished:
   }
 }
 
-template <bool PLAIN, bool LONG>
+template <Finish FINISH, bool LONG>
 int launch_part(SplitGemm& p, cudaStream_t stream) {
-  const int rc = allow_shared_memory<split_gemm_kernel<PLAIN, LONG>>(split_gemm_smem(LONG ? kMostChunks : 2));
+  const int rc = allow_shared_memory<split_gemm_kernel<FINISH, LONG>>(split_gemm_smem(LONG ? kMostChunks : 2));
   if (rc != TGT_OK) return rc;
   p.big_sums = (p.chunks + 1) / 2;
-  p.col_tiles = (p.cols + kCols - 1) / kCols;
+  constexpr int kTileColumns = FINISH == kGated ? kCols / 2 : kCols;
+  p.col_tiles = (p.cols + kTileColumns - 1) / kTileColumns;
   const int64_t tiles = (p.rows + kRows - 1) / kRows;
   const int resident = LONG ? 1 : 2;               // by shared memory, and tensor memory has 512 columns
   const int across = p.col_tiles * p.outputs;
   int64_t walkers = int64_t(sm_count()) * resident / across;
   if (walkers < 1) walkers = 1;
   if (walkers > tiles) walkers = tiles;
-  split_gemm_kernel<PLAIN, LONG><<<unsigned(walkers * across), kThreads, split_gemm_smem(p.chunks), stream>>>(p);
+  split_gemm_kernel<FINISH, LONG><<<unsigned(walkers * across), kThreads, split_gemm_smem(p.chunks), stream>>>(p);
   TGT_CHECK_CUDA(cudaGetLastError());
   return TGT_OK;
 }
@@ -347,11 +414,22 @@ int launch_split_gemm(const LinearRows& of, int* expired, cudaStream_t stream) {
       p.gate = p.add = nullptr;
     }
     const bool plain = is_plain(p);
-    const int rc = p.chunks > 2 ? (plain ? launch_part<true, true>(p, stream) : launch_part<false, true>(p, stream))
-                                : (plain ? launch_part<true, false>(p, stream) : launch_part<false, false>(p, stream));
+    const int rc = p.chunks > 2 ? (plain ? launch_part<kPlain, true>(p, stream) : launch_part<kAny, true>(p, stream))
+                                : (plain ? launch_part<kPlain, false>(p, stream) : launch_part<kAny, false>(p, stream));
     if (rc != TGT_OK) return rc;
   }
   return TGT_OK;
+}
+
+// one launch of a gated finish
+template <Finish FINISH>
+int launch_gated(SplitGemm& p, cudaStream_t stream) {
+  const int rc = expired_wait_word(&p.expired);
+  if (rc != TGT_OK) return rc;
+  p.sources = p.outputs = 1;
+  p.chunks = (p.red + kChunk - 1) / kChunk;
+  if (p.rows * p.red * 4 >= tc::kPrefetchFrom) p.ahead = p.chunks > 2 ? 1 : 2;
+  return p.chunks > 2 ? launch_part<FINISH, true>(p, stream) : launch_part<FINISH, false>(p, stream);
 }
 
 bool shape_supported(int reduce, int cols) {
@@ -359,6 +437,30 @@ bool shape_supported(int reduce, int cols) {
 }
 
 }  // namespace
+
+bool gated_in_one(int64_t rows, int reduce, int tile_columns) {
+  return (reduce + kChunk - 1) / kChunk <= kMostChunks && !few_rows(rows, tile_columns);
+}
+
+int linear_gated(const float* x, const float* w_gate, const float* w_up, int64_t rows, int reduce, int cols, int act, float* h,
+                 float* gate, float* up, cudaStream_t stream) {
+  SplitGemm p{};
+  p.a[0] = x; p.w[0] = w_gate; p.w[1] = w_up;
+  p.c[0] = h; p.c[1] = gate; p.c[2] = up;
+  p.rows = rows; p.red = reduce; p.cols = cols; p.act = act;
+  return launch_gated<kGated>(p, stream);
+}
+
+int linear_gated_grad(const float* dy, const float* w_down, const float* gate, const float* up, int64_t rows, int reduce, int cols,
+                      int act, float* dgate, float* dup, cudaStream_t stream) {
+  SplitGemm p{};
+  p.a[0] = dy; p.w[0] = w_down;
+  p.c[0] = dgate; p.c[1] = dup;
+  p.gate = gate; p.up = up;
+  p.rows = rows; p.red = reduce; p.cols = cols; p.act = act; p.transposed = true;
+  return launch_gated<kGatedGrad>(p, stream);
+}
+
 }  // namespace tgt
 
 extern "C" int tgt_linear_rows(const float* a, const float* w, const float* bias, int64_t rows, int reduce, int cols,

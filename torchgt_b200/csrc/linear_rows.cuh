@@ -1,6 +1,8 @@
 // The two kernels behind the products of narrow linear layers and the line between them.
 #pragma once
 
+#include <type_traits>
+
 #include "tgt_common.cuh"
 
 namespace tgt {
@@ -13,6 +15,56 @@ __device__ __forceinline__ float normal_cdf(float x) { return 0.5f * (1.f + erff
 __device__ __forceinline__ float gelu(float x) { return x * normal_cdf(x); }
 __device__ __forceinline__ float gelu_slope(float x) {
   return normal_cdf(x) + x * (0.39894228040143267794f * expf(-0.5f * x * x));
+}
+
+// 1 / (1 + exp(-x)) to about 2^-22: the power of two of x log2(e), whose rounding is put back to first order, and the
+// approximate reciprocal (1 unit).  0 below -87, where the quotient leaves the normal numbers, and for whatever a NaN makes of it.
+__device__ __forceinline__ float logistic(float x) {
+  constexpr float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299e-8f;      // their sum: log2(e)
+  const float y = fminf(fmaxf(x, -87.f), 87.f);
+  const float t = -y * kLog2e, rest = fmaf(-y, kLog2e, -t) - y * kLog2eRest;
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  e = fmaf(e, rest * 0.693147180559945309f, e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+  return x < -87.f ? 0.f : s;
+}
+// Activations of the gated block, silu among them, and with SLOPE their derivatives (of relu zero at zero).
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float gate_activation(float x, float& slope) {
+  if constexpr (ACT == TGT_ACT_SILU) {
+    const float s = logistic(x);
+    if (SLOPE) slope = s * (1.f + x * (1.f - s));
+    return x * s;
+  } else if constexpr (ACT == TGT_ACT_GELU) {
+    if (SLOPE) slope = gelu_slope(x);
+    return gelu(x);
+  } else {
+    if (SLOPE) slope = x <= 0.f ? 0.f : 1.f;
+    return relu(x);
+  }
+}
+// f(the activation as a constant), so that code over many values branches once
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+  if (act == TGT_ACT_SILU) f(std::integral_constant<int, TGT_ACT_SILU>());
+  else if (act == TGT_ACT_GELU) f(std::integral_constant<int, TGT_ACT_GELU>());
+  else f(std::integral_constant<int, TGT_ACT_RELU>());
+}
+// act(g) u of four values
+template <int ACT>
+__device__ __forceinline__ float4 gated(const float4& g, const float4& u) {
+  float unused;
+  return make_float4(gate_activation<ACT, false>(g.x, unused) * u.x, gate_activation<ACT, false>(g.y, unused) * u.y,
+                     gate_activation<ACT, false>(g.z, unused) * u.z, gate_activation<ACT, false>(g.w, unused) * u.w);
+}
+// and their gradients from that of the product: {dg, du}
+template <int ACT>
+__device__ __forceinline__ void gated_grad(const float4& d, const float4& g, const float4& u, float4& dg, float4& du) {
+  float4 s;
+  du.x = d.x * gate_activation<ACT, true>(g.x, s.x); du.y = d.y * gate_activation<ACT, true>(g.y, s.y);
+  du.z = d.z * gate_activation<ACT, true>(g.z, s.z); du.w = d.w * gate_activation<ACT, true>(g.w, s.w);
+  dg = make_float4(d.x * u.x * s.x, d.y * u.y * s.y, d.z * u.z * s.z, d.w * u.w * s.w);
 }
 
 // C_j[r][c] = f(sum_s sum_k A_s[r][k] B_sj[c][k] + bias_j[c]); one of `sources` (s) and `outputs` (j) is 1.
@@ -79,5 +131,13 @@ int linear_few_rows(const LinearRows& p, cudaStream_t stream);
 // chip better (us back to back, FMA / tensor cores, 64 x 64: 4,097 rows 4.2 / 6.3, 8,192 rows 6.0 / 6.5, 16,384 rows 10.7 / 6.5;
 // 64 x 128 at 8,192 rows, 128 tiles, 8.9 / 6.6).
 inline bool few_rows(int64_t rows, int cols) { return (rows + 127) / 128 * ((cols + 63) / 64) < 80; }
+
+// The gated block's products on the tensor cores with the gate in their finish (linear_mma.cu): gate = x w_gate^T, up = x w_up^T and
+// h = act(gate) up; dgate and dup from dh = dy w_down.  For reductions that are one launch and rows that fill the chip.
+bool gated_in_one(int64_t rows, int reduce, int tile_columns);
+int linear_gated(const float* x, const float* w_gate, const float* w_up, int64_t rows, int reduce, int cols, int act, float* h,
+                 float* gate, float* up, cudaStream_t stream);
+int linear_gated_grad(const float* dy, const float* w_down, const float* gate, const float* up, int64_t rows, int reduce, int cols,
+                      int act, float* dgate, float* dup, cudaStream_t stream);
 
 }  // namespace tgt
