@@ -566,20 +566,20 @@ TGT_API int tgt_embedding_sum_grad(const float* dout, const int64_t* ids, int64_
 /*
  * Root-mean-square norm of rows, with the residual addition in front of it: v = x + residual (NULL: v = x), y = v rstd weight
  * with rstd = 1 / sqrt(mean(v^2) + eps), in fp32 from tensors of `dtype` (TGT_F32 or TGT_BF16, all of the same); sum (may be
- * NULL) receives v, rstd (may be NULL) one fp32 value a row.  hidden is 1 to 16384 (TGT_ERR_UNSUPPORTED above).  Rows of
+ * NULL) receives v, rest (int8, may be NULL; of a bf16 sum) what its rounding took, rstd (may be NULL) one fp32 value a row.  hidden is 1 to 16384 (TGT_ERR_UNSUPPORTED above).  Rows of
  * whole 16-byte pieces from 16-byte boundaries on move in such pieces, others value by value.
  *   e4m3:     the same with y in 8 bits: scales [rows] = max(max |y| / 448, 2^-126) and values [rows, hidden] = y / scale, to
  *             the nearest e4m3 number.  A row with a NaN or an infinity has a NaN scale.
  *   backward: dx = rstd (dy weight - u mean(dy weight u)) + dsum with u = v rstd, dsum (may be NULL) the gradient of sum, v
- *             what the forward had as x or stored as sum; dweight [hidden] = sum over rows of dy u, fixed order.
+ *             what the forward had as x or stored as sum (with rest, or NULL); dweight [hidden] = sum over rows of dy u, fixed order.
  */
 TGT_API int tgt_rms_norm_fwd(const void* x, const void* residual, const void* weight, float eps, int64_t rows, int hidden,
-                             int dtype, void* sum, void* y, float* rstd, void* stream);
+                             int dtype, void* sum, void* rest, void* y, float* rstd, void* stream);
 TGT_API int tgt_rms_norm_e4m3(const void* x, const void* residual, const void* weight, float eps, int64_t rows, int hidden,
                               int dtype, void* sum, void* values, float* scales, void* stream);
 TGT_API int tgt_rms_norm_bwd_scratch_bytes(int64_t rows, int hidden, int dtype, size_t* bytes);
-TGT_API int tgt_rms_norm_bwd(const void* dy, const void* dsum, const void* v, const void* weight, const float* rstd,
-                             int64_t rows, int hidden, int dtype, void* dx, void* dweight, void* scratch,
+TGT_API int tgt_rms_norm_bwd(const void* dy, const void* dsum, const void* v, const void* rest, const void* weight,
+                             const float* rstd, int64_t rows, int hidden, int dtype, void* dx, void* dweight, void* scratch,
                              size_t scratch_bytes, void* stream);
 
 /*

@@ -59,17 +59,19 @@ def test_argument_checks_run_before_any_cuda_call():
     backwards = (ctypes.c_int32 * 3)(1, 4, 2)
     zero = (ctypes.c_int32 * 1)(0)
     # norm: types, sizes, null pointers
-    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 1, 64, 9, None, None, None, None) == 1
-    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, -1, 64, 0, None, None, None, None) == 1
-    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 1, 0, 0, None, None, None, None) == 1
-    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 1, 16385, 0, None, None, None, None) == 3
-    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 1, 64, 0, None, None, None, None) == 1
-    assert lib.tgt_rms_norm_fwd(16, None, 16, 0.0, 1, 64, 0, 16, 16, None, None) == 1          # a sum without a residual
-    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 0, 64, 0, None, None, None, None) == 0  # no rows
+    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 1, 64, 9, None, None, None, None, None) == 1
+    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, -1, 64, 0, None, None, None, None, None) == 1
+    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 1, 0, 0, None, None, None, None, None) == 1
+    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 1, 16385, 0, None, None, None, None, None) == 3
+    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 1, 64, 0, None, None, None, None, None) == 1
+    assert lib.tgt_rms_norm_fwd(16, None, 16, 0.0, 1, 64, 0, 16, None, 16, None, None) == 1          # a sum without a residual
+    assert lib.tgt_rms_norm_fwd(16, 16, 16, 0.0, 1, 64, 0, 16, 16, 16, None, None) == 1            # a rest of fp32
+    assert lib.tgt_rms_norm_fwd(16, 16, 16, 0.0, 1, 64, 1, None, 16, 16, None, None) == 1          # of no sum
+    assert lib.tgt_rms_norm_fwd(None, None, None, 0.0, 0, 64, 0, None, None, None, None, None) == 0  # no rows
     assert lib.tgt_rms_norm_e4m3(None, None, None, 0.0, 0, 64, 1, None, None, None, None) == 0
     assert lib.tgt_rms_norm_e4m3(16, None, 16, 0.0, 1, 64, 1, None, 16, None, None) == 1
     assert lib.tgt_rms_norm_bwd_scratch_bytes(10, 64, 0, None) == 1
-    assert lib.tgt_rms_norm_bwd(None, None, None, None, None, 1, 64, 0, None, None, None, 0, None) == 1
+    assert lib.tgt_rms_norm_bwd(None, None, None, None, None, None, 1, 64, 0, None, None, None, 0, None) == 1
     # bias: borders, sizes, null pointers
     assert lib.tgt_edge_position_bias(None, 0, 1, None, 0, 0, borders, 3, 1, None, 8, None, None, None) == 0
     assert lib.tgt_edge_position_bias(None, 1, 1, None, 0, 0, borders, 3, 1, None, 8, None, None, None) == 1

@@ -145,11 +145,11 @@ SIGNATURES = {
     "tgt_linear_wgrad": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_size_t,
                                  c_void_p]),
     "tgt_rms_norm_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p,
-                                 c_void_p]),
+                                 c_void_p, c_void_p]),
     "tgt_rms_norm_e4m3": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                   c_void_p]),
     "tgt_rms_norm_bwd_scratch_bytes": (c_int, [c_int64, c_int, c_int, POINTER(c_size_t)]),
-    "tgt_rms_norm_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,
+    "tgt_rms_norm_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,
                                  c_void_p, c_size_t, c_void_p]),
     "tgt_edge_position_bias": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_int, c_int, c_void_p,
                                        c_int, c_void_p, c_void_p, c_void_p]),

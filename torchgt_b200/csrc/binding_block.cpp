@@ -32,6 +32,7 @@ at::Tensor scratch_of(size_t bytes, const at::Tensor& like) {
 // Outputs: the normalised rows and, with a residual, x + residual.
 struct RmsNormRowsBackward : public torch::autograd::Node {
   SavedVariable normalised, weight, rstd;   // the norm's input: x, or the output x + residual
+  SavedVariable rest;                       // of a bf16 sum: what its rounding took
   bool with_residual = false;
   double eps = 0;
 
@@ -57,7 +58,7 @@ struct RmsNormRowsBackward : public torch::autograd::Node {
     const at::Tensor ds = with_residual ? grads[1] : at::Tensor();
     if (!grads[0].defined()) return {ds, ds, at::Tensor()};              // only x + residual was used, or nothing
     const at::Tensor v = with_residual ? normalised.unpack(shared_from_this()) : normalised.unpack();
-    const at::Tensor w = weight.unpack(), rstd_ = rstd.unpack();
+    const at::Tensor w = weight.unpack(), rstd_ = rstd.unpack(), rest_ = rest.unpack();
     if (at::GradMode::is_enabled() || at::isTensorSubclassLike(grads[0]) || (ds.defined() && at::isTensorSubclassLike(ds)))
       return recorded(grads[0], ds, v, w);
     const at::AutoDispatchBelowADInplaceOrView below;
@@ -69,7 +70,7 @@ struct RmsNormRowsBackward : public torch::autograd::Node {
     size_t bytes = 0;
     check(tgt_rms_norm_bwd_scratch_bytes(rows, int(hidden), type_code(v), &bytes));
     const at::Tensor scratch = scratch_of(bytes, dy);
-    check(tgt_rms_norm_bwd(ptr(dy), ptr(dsum), ptr(vc), ptr(wc), fptr(rstd_), rows, int(hidden), type_code(v), ptr(dx), ptr(dw),
+    check(tgt_rms_norm_bwd(ptr(dy), ptr(dsum), ptr(vc), ptr(rest_), ptr(wc), fptr(rstd_), rows, int(hidden), type_code(v), ptr(dx), ptr(dw),
                            scratch.data_ptr(), scratch.numel(), stream_of(dy)));
     return {dx, with_residual ? dx : at::Tensor(), dw};
   }
@@ -78,6 +79,7 @@ struct RmsNormRowsBackward : public torch::autograd::Node {
     normalised.reset_data();
     weight.reset_data();
     rstd.reset_data();
+    rest.reset_data();
   }
 };
 
@@ -97,14 +99,15 @@ std::pair<at::Tensor, std::optional<at::Tensor>> add_rms_norm(const at::Tensor& 
   const c10::cuda::CUDAGuard guard(x.device());
   const bool record = torch::autograd::compute_requires_grad(x, residual, w);
   const int64_t hidden = w.numel(), rows = x.numel() / hidden;
-  at::Tensor y, sum, rstd;
+  at::Tensor y, sum, rest, rstd;
   {
     const at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor xc = x.contiguous(), wc = w.contiguous(), rc = residual.defined() ? residual.contiguous() : residual;
     y = at::empty(x.sizes(), x.options());
     if (residual.defined() && (want_sum || record)) sum = at::empty(x.sizes(), x.options());
+    if (record && sum.defined() && x.scalar_type() == at::kBFloat16) rest = at::empty(x.sizes(), x.options().dtype(at::kChar));
     if (record) rstd = at::empty({rows}, x.options().dtype(at::kFloat));
-    check(tgt_rms_norm_fwd(ptr(xc), ptr(rc), ptr(wc), float(eps), rows, int(hidden), type_code(x), ptr(sum), ptr(y),
+    check(tgt_rms_norm_fwd(ptr(xc), ptr(rc), ptr(wc), float(eps), rows, int(hidden), type_code(x), ptr(sum), ptr(rest), ptr(y),
                            record ? fptr(rstd) : nullptr, stream_of(x)));
   }
   if (record) {
@@ -113,6 +116,7 @@ std::pair<at::Tensor, std::optional<at::Tensor>> add_rms_norm(const at::Tensor& 
     node->with_residual = residual.defined();
     node->eps = eps;
     node->rstd = SavedVariable(rstd, false);
+    node->rest = SavedVariable(rest, false);
     node->weight = SavedVariable(w, false);
     if (residual.defined()) {
       torch::autograd::set_history(variable_list{y, sum}, node);

@@ -4,8 +4,9 @@
 //   g = dy w,  u = v rstd:   dx = rstd (g - u mean(g u)) + dsum,  dw = sum over rows of dy u
 //   8 bits:  scale = max(max |y| / 448, 2^-126),  values = e4m3(y / scale)
 //
-// All of it in fp32, rounded once where it is stored; y comes from v before v is rounded for the residual stream, the
-// backward has the rounded one.  What is read and written bounds it: x and the residual in, y and the sum out; dy, the
+// All of it in fp32, rounded once where it is stored; y comes from v before v is rounded for the residual stream.  In bf16 the
+// forward can leave the next 8 bits of v beside the rounded sum for the backward: with the sum alone its rounding is in dw next
+// to dw's own (2.4e-3 from 64 bits in the 2-norm, with them 1.7e-3), for an eighth more bytes.  What is read and written bounds it: x and the residual in, y and the sum out; dy, the
 // residual stream's gradient and the sum in, dx out.  A row is held in registers between its sums and its results: by a group
 // of 8 to 32 lanes, or by a CTA where it is longer than a warp should hold.  Rows that are a whole number of 16-byte pieces
 // from 16-byte boundaries on move in such pieces, all others value by value.  The weight's gradient is summed per thread over
@@ -43,6 +44,35 @@ struct Piece<T, 1> {                    // one value
   __device__ __forceinline__ void clear() { raw = T(0.f); }
   __device__ __forceinline__ void unpack(float (&f)[1]) const { f[0] = widen(raw); }
   __device__ __forceinline__ static void store(T* row, int piece, const float (&f)[1]) { row[piece] = T(f[0]); }
+};
+
+// What a bf16 sum's rounding took from it, in steps of 2^-8 of its last place: the bits of v are (sum << 16) + (rest << 8),
+// rounded.  (The end of the range of a byte is a step nearer than it should be.)
+__device__ __forceinline__ int rest_of(float v) {
+  const int32_t bits = __float_as_int(v), sum = int32_t(__bfloat16_as_ushort(__float2bfloat16_rn(v))) << 16;
+  return min(max((bits - sum + 128) >> 8, -128), 127);
+}
+__device__ __forceinline__ float with_rest(float sum, int rest) { return __int_as_float(__float_as_int(sum) + rest * 256); }
+template <int VEC>
+__device__ __forceinline__ void store_rest(int8_t* row, int piece, const float (&v)[VEC]) {
+  if constexpr (VEC == 8) {
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i / 4] |= uint32_t(rest_of(v[i]) & 0xff) << (8 * (i % 4));
+    reinterpret_cast<uint2*>(row)[piece] = make_uint2(w[0], w[1]);
+  } else {
+    row[piece] = int8_t(rest_of(v[0]));
+  }
+}
+template <int VEC>
+struct Rest {                           // of a piece, as it is in memory
+  uint2 raw;
+  __device__ __forceinline__ void load(const int8_t* row, int piece) {
+    if constexpr (VEC == 8) raw = __ldg(reinterpret_cast<const uint2*>(row) + piece);
+    else raw.x = uint32_t(int32_t(row[piece]));
+  }
+  __device__ __forceinline__ void clear() { raw = make_uint2(0u, 0u); }
+  __device__ __forceinline__ int at(int i) const { return int(int8_t((i < 4 ? raw.x : raw.y) >> (8 * (i % 4)))); }
 };
 
 __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {   // +-448 where a value is larger, NaN stays NaN
@@ -114,6 +144,7 @@ struct RmsFwd {
   const T* residual;   // may be null
   const T* weight;
   T* sum;              // may be null
+  int8_t* rest;        // may be null (bf16)
   T* y;                // or, in 8 bits, values and scales
   uint8_t* values;
   float* scales;
@@ -167,6 +198,8 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_fwd_kernel(co
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[j][i] += f[i];
         if (p.sum != nullptr) Piece<T, VEC>::store(p.sum + r * p.hidden, c, v[j]);
+        if constexpr (sizeof(T) == 2)
+          if (p.rest != nullptr) store_rest<VEC>(p.rest + r * p.hidden, c, v[j]);
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) squares = fmaf(v[j][i], v[j][i], squares);
@@ -214,6 +247,7 @@ struct RmsBwd {
   const T* dy;
   const T* dsum;       // may be null
   const T* v;          // x, or the sum as it was stored
+  const int8_t* rest;  // of the sum; may be null (bf16)
   const T* weight;
   const float* rstd;
   T* dx;
@@ -240,7 +274,9 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_bwd_kernel(co
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[j][i] = 0.f;
   }
+  constexpr bool kRest = sizeof(T) == 2;
   Piece<T, VEC> next[PIECES], next_dy[PIECES], next_ds[PIECES];   // the next row, on its way
+  Rest<VEC> next_rest[kRest ? PIECES : 1];
   float next_rstd;
   auto load = [&](int64_t r) {
     next_rstd = r < p.rows ? __ldg(p.rstd + r) : 0.f;
@@ -249,10 +285,15 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_bwd_kernel(co
       const int c = at.first + j * at.step;
       if (r < p.rows && c < pieces) {
         next[j].load(p.v + r * p.hidden, c);
+        if constexpr (kRest) {
+          if (p.rest != nullptr) next_rest[j].load(p.rest + r * p.hidden, c);
+          else next_rest[j].clear();
+        }
         next_dy[j].load(p.dy + r * p.hidden, c);
         if (p.dsum != nullptr) next_ds[j].load(p.dsum + r * p.hidden, c);
       } else {
         next[j].clear();
+        if constexpr (kRest) next_rest[j].clear();
         next_dy[j].clear();
       }
     }
@@ -263,20 +304,29 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_bwd_kernel(co
     const int64_t r = r0 + at.row_of_cta;
     const bool live = r < p.rows;
     Piece<T, VEC> v[PIECES], dy[PIECES], ds[PIECES];
+    Rest<VEC> rest[kRest ? PIECES : 1];
     if (!kAhead) load(r);
     const float rstd = next_rstd;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
       v[j] = next[j];
+      if constexpr (kRest) rest[j] = next_rest[j];
       dy[j] = next_dy[j];
       ds[j] = next_ds[j];
     }
     if (kAhead) load(r + at.rows_at_once);
+    auto values = [&](int j, float (&f)[VEC]) {
+      v[j].unpack(f);
+      if constexpr (kRest) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = with_rest(f[i], rest[j].at(i));
+      }
+    };
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
       float f[VEC], d[VEC], g[VEC];
-      v[j].unpack(f);
+      values(j, f);
       dy[j].unpack(d);
       w[j].unpack(g);
 #pragma unroll
@@ -292,7 +342,7 @@ __global__ void __launch_bounds__(most_threads(LPR, VEC)) rms_norm_bwd_kernel(co
       const int c = at.first + j * at.step;
       if (!live || c >= pieces) continue;
       float f[VEC], d[VEC], g[VEC];
-      v[j].unpack(f);
+      values(j, f);
       dy[j].unpack(d);
       w[j].unpack(g);
 #pragma unroll
@@ -469,20 +519,20 @@ int launch_backward(RmsBwd<T> p, void* dweight, void* scratch, size_t scratch_by
 }
 
 template <typename T, bool E4M3>
-int forward(const void* x, const void* residual, const void* weight, float eps, int64_t rows, int hidden, void* sum, void* y,
-            void* values, float* scales, float* rstd, cudaStream_t stream) {
-  RmsFwd<T> p{static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight), static_cast<T*>(sum),
+int forward(const void* x, const void* residual, const void* weight, float eps, int64_t rows, int hidden, void* sum, int8_t* rest,
+            void* y, void* values, float* scales, float* rstd, cudaStream_t stream) {
+  RmsFwd<T> p{static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight), static_cast<T*>(sum), rest,
               static_cast<T*>(y), static_cast<uint8_t*>(values), scales, rstd, rows, hidden, eps};
-  return whole_pieces<T>(hidden, {x, residual, weight, sum, y, values}) ? launch_forward<T, kVec<T>, E4M3>(p, stream)
+  return whole_pieces<T>(hidden, {x, residual, weight, sum, rest, y, values}) ? launch_forward<T, kVec<T>, E4M3>(p, stream)
                                                                         : launch_forward<T, 1, E4M3>(p, stream);
 }
 
 template <typename T>
-int backward(const void* dy, const void* dsum, const void* v, const void* weight, const float* rstd, int64_t rows, int hidden,
+int backward(const void* dy, const void* dsum, const void* v, const int8_t* rest, const void* weight, const float* rstd, int64_t rows, int hidden,
              void* dx, void* dweight, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
-  RmsBwd<T> p{static_cast<const T*>(dy), static_cast<const T*>(dsum), static_cast<const T*>(v), static_cast<const T*>(weight),
-              rstd, static_cast<T*>(dx), nullptr, rows, hidden};
-  return whole_pieces<T>(hidden, {dy, dsum, v, weight, dx})
+  RmsBwd<T> p{static_cast<const T*>(dy), static_cast<const T*>(dsum), static_cast<const T*>(v), rest,
+              static_cast<const T*>(weight), rstd, static_cast<T*>(dx), nullptr, rows, hidden};
+  return whole_pieces<T>(hidden, {dy, dsum, v, rest, weight, dx})
              ? launch_backward<T, kVec<T>>(p, dweight, scratch, scratch_bytes, stream)
              : launch_backward<T, 1>(p, dweight, scratch, scratch_bytes, stream);
 }
@@ -491,7 +541,7 @@ int backward(const void* dy, const void* dsum, const void* v, const void* weight
 }  // namespace tgt
 
 extern "C" int tgt_rms_norm_fwd(const void* x, const void* residual, const void* weight, float eps, int64_t rows, int hidden,
-                                int dtype, void* sum, void* y, float* rstd, void* stream_) {
+                                int dtype, void* sum, void* rest, void* y, float* rstd, void* stream_) {
   using namespace tgt;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const int rc = check_rows(rows, hidden, dtype);
@@ -499,9 +549,10 @@ extern "C" int tgt_rms_norm_fwd(const void* x, const void* residual, const void*
   if (rows == 0) return TGT_OK;
   TGT_CHECK_ARG(x && weight && y, "x, weight and y must not be null");
   TGT_CHECK_ARG(sum == nullptr || residual != nullptr, "sum without a residual");
-  return dtype == TGT_F32 ? forward<float, false>(x, residual, weight, eps, rows, hidden, sum, y, nullptr, nullptr, rstd, stream)
-                          : forward<__nv_bfloat16, false>(x, residual, weight, eps, rows, hidden, sum, y, nullptr, nullptr, rstd,
-                                                          stream);
+  TGT_CHECK_ARG(rest == nullptr || (sum != nullptr && dtype == TGT_BF16), "rest is of a bf16 sum");
+  return dtype == TGT_F32 ? forward<float, false>(x, residual, weight, eps, rows, hidden, sum, nullptr, y, nullptr, nullptr, rstd, stream)
+                          : forward<__nv_bfloat16, false>(x, residual, weight, eps, rows, hidden, sum, static_cast<int8_t*>(rest), y,
+                                                          nullptr, nullptr, rstd, stream);
 }
 
 extern "C" int tgt_rms_norm_e4m3(const void* x, const void* residual, const void* weight, float eps, int64_t rows, int hidden,
@@ -514,8 +565,9 @@ extern "C" int tgt_rms_norm_e4m3(const void* x, const void* residual, const void
   TGT_CHECK_ARG(x && weight && values && scales, "x, weight, values and scales must not be null");
   TGT_CHECK_ARG(sum == nullptr || residual != nullptr, "sum without a residual");
   return dtype == TGT_F32
-             ? forward<float, true>(x, residual, weight, eps, rows, hidden, sum, nullptr, values, scales, nullptr, stream)
-             : forward<__nv_bfloat16, true>(x, residual, weight, eps, rows, hidden, sum, nullptr, values, scales, nullptr, stream);
+             ? forward<float, true>(x, residual, weight, eps, rows, hidden, sum, nullptr, nullptr, values, scales, nullptr, stream)
+             : forward<__nv_bfloat16, true>(x, residual, weight, eps, rows, hidden, sum, nullptr, nullptr, values, scales, nullptr,
+                                           stream);
 }
 
 extern "C" int tgt_rms_norm_bwd_scratch_bytes(int64_t rows, int hidden, int dtype, size_t* bytes) {
@@ -535,8 +587,8 @@ extern "C" int tgt_rms_norm_bwd_scratch_bytes(int64_t rows, int hidden, int dtyp
   return TGT_OK;
 }
 
-extern "C" int tgt_rms_norm_bwd(const void* dy, const void* dsum, const void* v, const void* weight, const float* rstd,
-                                int64_t rows, int hidden, int dtype, void* dx, void* dweight, void* scratch,
+extern "C" int tgt_rms_norm_bwd(const void* dy, const void* dsum, const void* v, const void* rest, const void* weight,
+                                const float* rstd, int64_t rows, int hidden, int dtype, void* dx, void* dweight, void* scratch,
                                 size_t scratch_bytes, void* stream_) {
   using namespace tgt;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -548,7 +600,9 @@ extern "C" int tgt_rms_norm_bwd(const void* dy, const void* dsum, const void* v,
     return TGT_OK;
   }
   TGT_CHECK_ARG(dy && v && weight && rstd && dx, "dy, v, weight, rstd and dx must not be null");
-  return dtype == TGT_F32 ? backward<float>(dy, dsum, v, weight, rstd, rows, hidden, dx, dweight, scratch, scratch_bytes, stream)
-                          : backward<__nv_bfloat16>(dy, dsum, v, weight, rstd, rows, hidden, dx, dweight, scratch, scratch_bytes,
-                                                    stream);
+  TGT_CHECK_ARG(rest == nullptr || dtype == TGT_BF16, "rest is of a bf16 sum");
+  return dtype == TGT_F32
+             ? backward<float>(dy, dsum, v, nullptr, weight, rstd, rows, hidden, dx, dweight, scratch, scratch_bytes, stream)
+             : backward<__nv_bfloat16>(dy, dsum, v, static_cast<const int8_t*>(rest), weight, rstd, rows, hidden, dx, dweight, scratch,
+                                       scratch_bytes, stream);
 }
