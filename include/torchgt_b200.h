@@ -609,6 +609,7 @@ TGT_API int tgt_edge_position_bias_grad(const float* dbias, const uint16_t* buck
  *                in bf16 the upper 16 bits of their fp32 sums, and in low [rows, mid] the next 8 bits of both (gate's in the
  *                lower byte); in fp32 the sums, and low is not used
  *   output:      y; add [rows, out] may be NULL and must not overlap y
+ *   block:       the two in one call, in bf16 the second as the first's dependent
  *   hidden_grad: from dy [rows, out], dh = dy w_down: dgate = dh up act'(gate) and dup = dh act(gate)
  *   input_grad:  dx = dgate w_gate + dup w_up
  *   weight_grad: dw[i] [out_features, in_features] = dy[i]^T x for `count` 1 or 2 (host arrays of pointers): (dgate, dup) with x,
@@ -621,6 +622,9 @@ TGT_API int tgt_gated_hidden(const void* x, const void* w_gate, const void* w_up
                              int dtype, void* h, void* gate, void* up, void* low, void* stream);
 TGT_API int tgt_gated_output(const void* h, const void* w_down, const void* add, int64_t rows, int mid, int out, int dtype,
                              void* y, void* stream);
+TGT_API int tgt_gated_block(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* add, int64_t rows,
+                            int in, int mid, int out, int act, int dtype, void* h, void* gate, void* up, void* low, void* y,
+                            void* stream);
 TGT_API int tgt_gated_hidden_grad(const void* dy, const void* w_down, const void* gate, const void* up, const void* low,
                                   int64_t rows, int out, int mid, int act, int dtype, void* dgate, void* dup, void* stream);
 TGT_API int tgt_gated_input_grad(const void* dgate, const void* dup, const void* w_gate, const void* w_up, int64_t rows, int mid,

@@ -361,8 +361,8 @@ at::Tensor gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const a
                                stream));
       return y;
     }
-    check(tgt_gated_hidden(ptr(xc), ptr(wgc), ptr(wuc), rows, int(in), int(mid), act, type, ptr(h), ptr(g), ptr(u), ptr(l), stream));
-    check(tgt_gated_output(ptr(h), ptr(wdc), ptr(rc), rows, int(mid), int(out), type, ptr(y), stream));
+    check(tgt_gated_block(ptr(xc), ptr(wgc), ptr(wuc), ptr(wdc), ptr(rc), rows, int(in), int(mid), int(out), act, type, ptr(h), ptr(g),
+                          ptr(u), ptr(l), ptr(y), stream));
   }
   if (record) {
     auto node = std::shared_ptr<GatedFeedForwardBackward>(new GatedFeedForwardBackward(), torch::autograd::deleteNode);

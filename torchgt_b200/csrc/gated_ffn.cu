@@ -78,7 +78,7 @@ struct Cut {
 };
 
 template <int BN, bool PAIR, bool A_MN, bool B_MN, gemm::Finish FINISH>
-int launch(const Gemm& p, int walkers, cudaStream_t stream) {
+int launch(const Gemm& p, int walkers, cudaStream_t stream, bool chained = false) {
   constexpr int kSmem = gemm::smem_bytes(PAIR ? BN / 2 : BN, FINISH);
   TGT_RETURN_IF(allow_shared_memory<gemm::gemm_kernel<BN, PAIR, A_MN, B_MN, FINISH>>(kSmem));
   cudaLaunchConfig_t cfg = {};
@@ -86,13 +86,18 @@ int launch(const Gemm& p, int walkers, cudaStream_t stream) {
   cfg.blockDim = dim3(gemm::kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
   if (PAIR) {
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = 2;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (chained) {               // the dependent of the kernel in front of it, one of this entry point's
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
   }
   TGT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm::gemm_kernel<BN, PAIR, A_MN, B_MN, FINISH>, p));
   return TGT_OK;
@@ -152,14 +157,14 @@ Plan plan_for(int products, int64_t m, int columns, int narrowest, int chunks, d
 }
 
 template <int BN, bool PAIR, bool A_MN, bool B_MN, gemm::Finish FINISH>
-int launch_cut(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+int launch_cut(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cudaStream_t stream, bool chained) {
   if (q.scratch() > 0) {
     if (scratch == nullptr || scratch_bytes < q.scratch())
       return set_error(TGT_ERR_WORKSPACE, "scratch holds %zu bytes, %zu needed", scratch_bytes, q.scratch());
     TGT_CHECK_ARG(aligned16(scratch), "scratch must be 16-byte aligned");
     p.partial = static_cast<float*>(scratch);
   }
-  TGT_RETURN_IF(launch<BN, PAIR, A_MN, B_MN, FINISH>(p, q.walkers, stream));
+  TGT_RETURN_IF(launch<BN, PAIR, A_MN, B_MN, FINISH>(p, q.walkers, stream, chained));
   if constexpr (A_MN) {
     if (q.shared() == 0) return TGT_OK;
     const gemm::SumParts s{p.partial, {p.out[0], p.out[1]}, p.m, p.n, q.m_tiles, q.n_tiles,
@@ -172,15 +177,15 @@ int launch_cut(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cuda
   return TGT_OK;
 }
 template <bool A_MN, bool B_MN, gemm::Finish FINISH>
-int launch_plan(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+int launch_plan(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cudaStream_t stream, bool chained = false) {
   q.into(p);
   if (q.cut.pair) {
-    if (q.cut.bn == 256) return launch_cut<256, true, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
-    return launch_cut<128, true, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
+    if (q.cut.bn == 256) return launch_cut<256, true, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream, chained);
+    return launch_cut<128, true, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream, chained);
   }
-  if (q.cut.bn == 256) return launch_cut<256, false, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
-  if (q.cut.bn == 128) return launch_cut<128, false, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
-  if constexpr (FINISH != gemm::kGated) return launch_cut<64, false, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream);
+  if (q.cut.bn == 256) return launch_cut<256, false, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream, chained);
+  if (q.cut.bn == 128) return launch_cut<128, false, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream, chained);
+  if constexpr (FINISH != gemm::kGated) return launch_cut<64, false, A_MN, B_MN, FINISH>(q, p, scratch, scratch_bytes, stream, chained);
   return set_error(TGT_ERR_INVALID, "no tile of %d columns", q.cut.bn);
 }
 
@@ -274,10 +279,11 @@ extern "C" int tgt_gated_hidden(const void* x, const void* w_gate, const void* w
   return launch_plan<false, false, gemm::kGated>(q, p, nullptr, 0, stream);
 }
 
-extern "C" int tgt_gated_output(const void* h, const void* w_down, const void* add, int64_t rows, int mid, int out, int dtype,
-                                void* y, void* stream_) {
-  using namespace tgt;
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+namespace tgt {
+namespace {
+
+int gated_output(const void* h, const void* w_down, const void* add, int64_t rows, int mid, int out, int dtype, void* y, cudaStream_t stream,
+                 bool chained) {
   TGT_RETURN_IF(check_widths(rows, mid, out, dtype, TGT_ACT_SILU));
   if (rows == 0) return TGT_OK;
   TGT_CHECK_ARG(h && w_down && y, "h, w_down and y must not be null");
@@ -298,8 +304,23 @@ extern "C" int tgt_gated_output(const void* h, const void* w_down, const void* a
   p.read[0] = words(add);
   p.m = int(rows); p.n = out;
   p.source_chunks = q.chunks;
-  return add != nullptr ? launch_plan<false, false, gemm::kPlus>(q, p, nullptr, 0, stream)
-                        : launch_plan<false, false, gemm::kPlain>(q, p, nullptr, 0, stream);
+  return add != nullptr ? launch_plan<false, false, gemm::kPlus>(q, p, nullptr, 0, stream, chained)
+                        : launch_plan<false, false, gemm::kPlain>(q, p, nullptr, 0, stream, chained);
+}
+
+}  // namespace
+}  // namespace tgt
+
+extern "C" int tgt_gated_output(const void* h, const void* w_down, const void* add, int64_t rows, int mid, int out, int dtype,
+                                void* y, void* stream) {
+  return tgt::gated_output(h, w_down, add, rows, mid, out, dtype, y, static_cast<cudaStream_t>(stream), false);
+}
+
+extern "C" int tgt_gated_block(const void* x, const void* w_gate, const void* w_up, const void* w_down, const void* add, int64_t rows,
+                               int in, int mid, int out, int act, int dtype, void* h, void* gate, void* up, void* low, void* y,
+                               void* stream) {
+  const int rc = tgt_gated_hidden(x, w_gate, w_up, rows, in, mid, act, dtype, h, gate, up, low, stream);
+  return rc != TGT_OK ? rc : tgt::gated_output(h, w_down, add, rows, mid, out, dtype, y, static_cast<cudaStream_t>(stream), true);
 }
 
 extern "C" int tgt_gated_hidden_grad(const void* dy, const void* w_down, const void* gate, const void* up, const void* low,

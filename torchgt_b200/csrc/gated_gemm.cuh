@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     tma::barriers_ready();
   }
   __syncwarp();
+  if (FINISH == kGated) release_dependents();            // the product of h, if it was launched so
   if (warp == kFinishWarps + 1) allocate<PAIR, 2 * BN>(s_tmem);
   tc::fence_before_barrier();
   __syncthreads();
@@ -249,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     uint32_t phase = 1;                                  // an empty ring's stages count as taken
     const uint32_t full = first_ctas<PAIR>(tc::smem_address(s_full));
     bool ok = true;
+    dependent_wait();                                    // for h
     while (ok && work.next()) {
       int m_tile, n_tile;
       place(p.m_tiles, p.n_tiles, work.tile, m_tile, n_tile);

@@ -13,6 +13,7 @@
 // the rows it walks, then over a CTA's groups and over the CTAs in a fixed order: no atomics, the same bits every time.
 #include <cuda_fp8.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "tgt_common.cuh"
@@ -457,15 +458,32 @@ bool with_shape(const Shape& s, F&& f) {
   return false;
 }
 
-// CTAs that are resident together, but no more than have rows
+// CTAs to walk the rows, no more than have any: of the backward no more than are resident together, so that all end at one
+// time, nor than leave few rows of partial sums.
 int grid_of(const Shape& s, int64_t rows, int ctas_per_sm) {
   const int64_t at_once = s.lpr == 0 ? 1 : kGroupThreads / s.lpr;
   const int64_t want = (rows + at_once - 1) / at_once, most = int64_t(sm_count()) * ctas_per_sm;
   return int(want < most ? want : most);
 }
 int forward_grid(const Shape& s, int64_t rows) { return grid_of(s, rows, 2048 / s.threads); }
-// each CTA leaves a row of partial sums: fewer of them
-int backward_grid(const Shape& s, int64_t rows) { return grid_of(s, rows, 1024 / s.threads); }
+int most_backward_grid(const Shape& s, int64_t rows) { return grid_of(s, rows, 1024 / s.threads); }
+// resident CTAs of a kernel on an SM, asked once for each device and block size
+template <auto Kernel>
+int resident(int threads, int smem) {
+  static std::atomic<int> cache[kMaxDevices][1024 / 32 + 1] = {};
+  const int dev = current_device();
+  if (dev < 0) return 1;
+  std::atomic<int>& known = cache[dev][threads / 32];
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, threads, smem) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    known.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 int check_rows(int64_t rows, int hidden, int dtype) {
   TGT_CHECK_ARG(dtype == TGT_F32 || dtype == TGT_BF16, "dtype must be TGT_F32 or TGT_BF16");
@@ -501,15 +519,20 @@ int launch_forward(const RmsFwd<T>& p, cudaStream_t stream) {
 template <typename T, int VEC>
 int launch_backward(RmsBwd<T> p, void* dweight, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
   const Shape s = shape_of(p.hidden, VEC);
-  const int grid = backward_grid(s, p.rows);
+  int grid = most_backward_grid(s, p.rows);
   if (scratch == nullptr || scratch_bytes < size_t(grid) * p.hidden * sizeof(float))
     return set_error(TGT_ERR_WORKSPACE, "scratch holds %zu bytes, %zu needed", scratch_bytes, size_t(grid) * p.hidden * sizeof(float));
   p.partial = static_cast<float*>(scratch);
   const size_t smem = s.lpr == 0 ? 0 : size_t(kGroupThreads / 32) * p.hidden * sizeof(float);
   const bool built = with_shape(s, [&](auto lpr, auto pieces) {
     constexpr int kLpr = decltype(lpr)::value, kPieces = decltype(pieces)::value;
-    if constexpr (VEC == 1 || kPieces * kVec<T> <= 32)
+    if constexpr (VEC == 1 || kPieces * kVec<T> <= 32) {
+      if (s.lpr == 0) {
+        const int all = sm_count() * resident<rms_norm_bwd_kernel<T, VEC, kLpr, kPieces>>(s.threads, 0);
+        if (grid > all) grid = all;
+      }
       rms_norm_bwd_kernel<T, VEC, kLpr, kPieces><<<grid, s.threads, smem, stream>>>(p);
+    }
   });
   if (!built) return set_error(TGT_ERR_UNSUPPORTED, "no kernel for hidden=%d", p.hidden);
   TGT_CHECK_CUDA(cudaGetLastError());
@@ -578,9 +601,9 @@ extern "C" int tgt_rms_norm_bwd_scratch_bytes(int64_t rows, int hidden, int dtyp
   const size_t size = dtype == TGT_F32 ? 4 : 2;
   const int vec = int(16 / size);
   // whether the pointers allow whole pieces is not known yet
-  int grid = backward_grid(shape_of(hidden, 1), rows);
+  int grid = most_backward_grid(shape_of(hidden, 1), rows);
   if (hidden % vec == 0) {
-    const int other = backward_grid(shape_of(hidden, vec), rows);
+    const int other = most_backward_grid(shape_of(hidden, vec), rows);
     grid = other > grid ? other : grid;
   }
   *bytes = size_t(grid) * hidden * sizeof(float);
