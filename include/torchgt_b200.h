@@ -567,7 +567,8 @@ TGT_API int tgt_embedding_sum_grad(const float* dout, const int64_t* ids, int64_
  * Root-mean-square norm of rows, with the residual addition in front of it: v = x + residual (NULL: v = x), y = v rstd weight
  * with rstd = 1 / sqrt(mean(v^2) + eps), in fp32 from tensors of `dtype` (TGT_F32 or TGT_BF16, all of the same); sum (may be
  * NULL) receives v, rest (int8, may be NULL; of a bf16 sum) what its rounding took, rstd (may be NULL) one fp32 value a row.  hidden is 1 to 16384 (TGT_ERR_UNSUPPORTED above).  Rows of
- * whole 16-byte pieces from 16-byte boundaries on move in such pieces, others value by value.
+ * whole 16-byte pieces from 16-byte boundaries on move in such pieces, others value by value.  What is written must not overlap
+ * what is read.
  *   e4m3:     the same with y in 8 bits: scales [rows] = max(max |y| / 448, 2^-126) and values [rows, hidden] = y / scale, to
  *             the nearest e4m3 number.  A row with a NaN or an infinity has a NaN scale.
  *   backward: dx = rstd (dy weight - u mean(dy weight u)) + dsum with u = v rstd, dsum (may be NULL) the gradient of sum, v

@@ -143,3 +143,34 @@ def test_a_captured_step_next_to_an_eager_one():
     torch.cuda.synchronize()
     for a, b, c in zip(want, eager, held):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_traced_transformed_and_compiled_calls_are_operations():
+    """Under vmap, forward-mode derivatives, torch.func.grad and the tracer the operators are torch's operations, with the same
+    values within the types' tolerance."""
+    from torchgt_b200 import edge_position_bias, gated_feed_forward
+    from torchgt_b200.rms_norm import add_rms_norm
+    gen = torch.Generator().manual_seed(9)
+    x, r, dx = (torch.randn(4, 30, HIDDEN, generator=gen).cuda() for _ in range(3))
+    w = torch.randn(HIDDEN, generator=gen).cuda()
+    wg, wu, wd = (torch.randn(HIDDEN, HIDDEN, generator=gen).cuda() / 8 for _ in range(3))
+    edges = torch.randint(0, 30, (2, 100), generator=gen).cuda()
+    tables = torch.randn(4, 32, HEADS, generator=gen).cuda()
+    norm = lambda a, b: add_rms_norm(a, b, w, EPS)[0]                            # noqa: E731
+    ffn = lambda a, b: gated_feed_forward(a, wg, wu, wd, "silu", b)              # noqa: E731
+    for f in (norm, ffn):
+        want = f(x, r)
+        assert rel_err(torch.func.vmap(f)(x, r), want) <= TOL_F32
+        assert rel_err(torch.jit.trace(f, (x, r))(x, r), want) <= TOL_F32
+        value, tangent = torch.func.jvp(f, (x, r), (dx, torch.zeros_like(dx)))
+        step = 2.0 ** -7                        # the difference of two fp32 results, each 1e-6 off, over this; third derivatives below 64
+        slope = (f(x + step * dx, r).double() - f(x - step * dx, r).double()) / (2 * step)
+        assert rel_err(value, want) <= TOL_F32 and rel_err(tangent, slope) <= 1e-6 / step + 64 * step * step
+        leaf = x.clone().requires_grad_()
+        g, = torch.autograd.grad(f(leaf, r).square().sum(), [leaf])
+        assert rel_err(torch.func.grad(lambda a: f(a, r).square().sum())(x), g) <= 5 * TOL_F32
+    want = torch.stack([edge_position_bias(t, edges) for t in tables])
+    assert torch.equal(torch.func.vmap(lambda t: edge_position_bias(t, edges))(tables), want)
+    assert torch.equal(torch.jit.trace(lambda t: edge_position_bias(t, edges), (tables[0],), check_trace=False)(tables[0]), want[0])
+    value, tangent = torch.func.jvp(lambda t: edge_position_bias(t, edges), (tables[0],), (tables[1],))
+    assert torch.equal(value, want[0]) and torch.equal(tangent, want[1])

@@ -180,17 +180,20 @@ struct EdgePositionBiasBackward : public torch::autograd::Node {
   void release_variables() override { buckets.reset_data(); }
 };
 
+// The caller has checked types and shapes; what is left are wrappers of torch.func, dual numbers and the like.
+bool edge_position_bias_covers(const at::Tensor& table, const at::Tensor& edge_index, const std::optional<at::Tensor>& positions) {
+  auto ids = [&](const at::Tensor& t) { return plain(t, table.device(), at::kLong) || plain(t, table.device(), at::kInt); };
+  return table.defined() && plain(table, table.device(), at::kFloat) && ids(edge_index) && (!positions.has_value() || ids(*positions));
+}
+
 // The caller has checked types, shapes and the borders.
 at::Tensor edge_position_bias(const at::Tensor& table, const at::Tensor& edge_index, const std::optional<at::Tensor>& positions,
                               const std::vector<int32_t>& borders, bool both_ways) {
-  const at::Device device = table.device();
-  auto whole = [&](const at::Tensor& t) {
-    return t.is_cuda() && t.device() == device && (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt);
-  };
-  TORCH_CHECK(plain(table, device, at::kFloat) && table.dim() == 2 && whole(edge_index) && edge_index.dim() == 2 &&
-                  edge_index.size(0) == 2 && (!positions.has_value() || (whole(*positions) && positions->dim() == 1)) &&
+  TORCH_CHECK(edge_position_bias_covers(table, edge_index, positions) && table.dim() == 2 && edge_index.dim() == 2 &&
+                  edge_index.size(0) == 2 && (!positions.has_value() || positions->dim() == 1) &&
                   table.size(0) == int64_t(borders.size() + 1) * (both_ways ? 2 : 1),
               "edge_position_bias: tensors that the kernels do not cover");
+  const at::Device device = table.device();
   const c10::cuda::CUDAGuard guard(device);
   const int64_t edges = edge_index.size(1), heads = table.size(1);
   const bool record = torch::autograd::compute_requires_grad(table);
@@ -388,6 +391,7 @@ void bind_block(pybind11::module_& m) {
   m.def("rms_norm_covers", &rms_norm_covers);
   m.def("add_rms_norm", &add_rms_norm, Unlocked());
   m.def("rms_norm_e4m3", &rms_norm_e4m3, Unlocked());
+  m.def("edge_position_bias_covers", &edge_position_bias_covers);
   m.def("edge_position_bias", &edge_position_bias, Unlocked());
   m.def("gated_feed_forward_covers", &gated_feed_forward_covers);
   m.def("gated_feed_forward", &gated_feed_forward, Unlocked());

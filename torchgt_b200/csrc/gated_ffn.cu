@@ -282,8 +282,8 @@ extern "C" int tgt_gated_hidden(const void* x, const void* w_gate, const void* w
 namespace tgt {
 namespace {
 
-int gated_output(const void* h, const void* w_down, const void* add, int64_t rows, int mid, int out, int dtype, void* y, cudaStream_t stream,
-                 bool chained) {
+int gated_output(const void* h, const void* w_down, const void* add, int64_t rows, int mid, int out, int dtype, void* y,
+                 cudaStream_t stream, bool chained) {
   TGT_RETURN_IF(check_widths(rows, mid, out, dtype, TGT_ACT_SILU));
   if (rows == 0) return TGT_OK;
   TGT_CHECK_ARG(h && w_down && y, "h, w_down and y must not be null");

@@ -1,15 +1,22 @@
 // bf16 products with fp32 sums for the gated feed-forward block (gated_ffn.cu): one kernel whose operands lie either way
-// round and whose finish is one of four.  Of weight gradients, which are long sums for few results, the last tiles, those that do not
-// fill all SMs, are shared out along k: their parts go to scratch and a second kernel adds them.
+// round and whose finish is one of four.  Of weight gradients, which are long sums for few results, the last tiles, those
+// that do not fill all SMs, are shared out along k: their parts go to scratch and a second kernel adds them.
 //
 //   D[m][n] = sum over k of A[m][k] B[n][k]
 //
 // A CTA takes tiles of 128 x BN, or two CTAs (PAIR) tiles of 256 x BN together: each has 128 rows of A and of the sums and
-// brings in half of B's rows, and the first issues the products for both, so a tile costs a third less of what the L2 hands out.  One warp brings the operands in by TMA, 64 of k at a time, into a ring of stages; one
-// issues tcgen05.mma on them, four a stage; eight finish the tile before from the other half of the tensor memory: 32 rows
-// and half of the columns each, 32 columns at a time.  A lane reads a row of the sums; what is read and written of global memory
-// goes by four lanes to 64 bytes of a row, and 4 KB of shared memory per warp stand between the two.  An operand is `k`-major (rows of k, as x and the forward's weights) or `mn`-major (rows of m or n: what the
-// gradients read without a transposed copy).
+// brings in half of B's rows, and the first issues the products for both, so a tile costs a third less of what the L2 hands
+// out.  One warp brings the operands in by TMA, 64 of k at a time, into a ring of stages; one issues tcgen05.mma on them,
+// four a stage; eight finish the tile before from the other half of the tensor memory: 32 rows and half of the columns
+// each, 32 columns at a time.  A lane reads a row of the sums; what is read and written of global memory goes by four lanes
+// to 64 bytes of a row, and 4 KB of shared memory per warp stand between the two.  An operand is `k`-major (rows of k, as x
+// and the forward's weights) or `mn`-major (rows of m or n: what the gradients read without a transposed copy).
+//
+// TFLOP/s at 1.4 to 1.9 GHz (library's product in brackets where there is one): y of 18,944 rows 4,096 x 2,048 1,555
+// (1,580); of 8,191 rows 5,632 x 2,048, 3.5 rounds of tiles in 4, 1,391 (1,540); h of 8,191 rows 2,048 x 5,632 1,540, with
+// what is kept 16,384 rows 1,024 x 2,816 1,170 (370 MB out); dgate and dup 800 (460 MB in and out); dx 1,400; the weights'
+// gradients 1,380.  What bounds them: the tensor cores, and under a long run the power cap; with kept or read matrices the
+// bytes of the finish next to what the L2 hands out for the ring.
 #pragma once
 
 #include "linear_rows.cuh"
@@ -31,7 +38,8 @@ enum Finish {
 };
 
 struct Gemm {
-  CUtensorMap a[2], b[2];      // of two sources (k one after the other), or a of two products of one b, or (kGated) b of the two projections
+  // of two sources (k one after the other), or a of two products of one b, or (kGated) b of the two projections
+  CUtensorMap a[2], b[2];
   uint16_t* out[4];            // [m][n]; of two products out[0] and out[1]
   const uint16_t* read[3];     // kPlus: add; kGatedGrad: the three that were kept
   float* partial;              // [walkers + tiles that are shared][CTAs of a tile][BN][kTileM]
@@ -184,15 +192,17 @@ __device__ __forceinline__ float activate(float x, float& slope) {
     return relu(x);
   }
 }
-// How the two projections are kept for the gradients: the upper 16 bits of each fp32 sum, and the 8 bits below those of both in
-// a third word.  Their rounding would be in every gradient, next to the roundings of dgate, dup and the result that cannot be avoided: kept in
-// bf16 dx, dWg and dWu are 3.1e-3 from 64 bits (2-norm), with the 8 bits 2.4e-3, rounding the results alone 1.7e-3.
+// How the two projections are kept for the gradients: the upper 16 bits of each fp32 sum, and the 8 bits below those of
+// both in a third word.  Their rounding would be in every gradient, next to the roundings of dgate, dup and the result that
+// cannot be avoided: kept in bf16 dx, dWg and dWu are 3.1e-3 from 64 bits (2-norm), with the 8 bits 2.3e-3, rounding the
+// results alone 1.7e-3.
 __device__ __forceinline__ uint32_t upper_pair(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
 __device__ __forceinline__ uint32_t lower_pair(float g0, float u0, float g1, float u1) {
   return __byte_perm(__byte_perm(__float_as_uint(g0), __float_as_uint(u0), 0x0051),
                      __byte_perm(__float_as_uint(g1), __float_as_uint(u1), 0x0051), 0x5410);
 }
-// the gate's (which 0) or the up projection's (1) value i of a pair; the byte at the end, of which nothing is known, is the one before it again
+// the gate's (which 0) or the up projection's (1) value i of a pair; the last byte, of which nothing is known, is the one before
+// it again
 __device__ __forceinline__ float whole(uint32_t upper, uint32_t lower, int i, int which) {
   return __uint_as_float(__byte_perm(lower, upper, i == 0 ? (which == 0 ? 0x5400 : 0x5411) : (which == 0 ? 0x7622 : 0x7633)));
 }
@@ -239,6 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   if constexpr (PAIR) pair_barrier();
   tc::fence_after_barrier();
   const uint32_t tmem = *s_tmem;
+  dependent_wait();                                      // for h; before any wait here that has a limit
   Work work(p, walker, gridDim.x / kCtas);
 
   // The two warps that feed the tensor cores go through their loops together and elect a lane where something is issued: in code that a
@@ -250,7 +261,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     uint32_t phase = 1;                                  // an empty ring's stages count as taken
     const uint32_t full = first_ctas<PAIR>(tc::smem_address(s_full));
     bool ok = true;
-    dependent_wait();                                    // for h
     while (ok && work.next()) {
       int m_tile, n_tile;
       place(p.m_tiles, p.n_tiles, work.tile, m_tile, n_tile);
@@ -546,7 +556,8 @@ __global__ void __launch_bounds__(256 * SLICES) sum_parts_kernel(const SumParts 
   __shared__ float s_block[SLICES][64][33];
   const int warp = threadIdx.x / 32 % 8, slice = threadIdx.x / 256, lane = threadIdx.x % 32;
   const int shared_tile = blockIdx.x, r0 = blockIdx.y % (kTileRows / 32) * 32, c0 = blockIdx.y / (kTileRows / 32) * 64;
-  const int64_t all = (int64_t(p.m_tiles) * p.n_tiles - p.whole) * p.chunks, begin = int64_t(shared_tile) * p.chunks, end = begin + p.chunks;
+  const int64_t all = (int64_t(p.m_tiles) * p.n_tiles - p.whole) * p.chunks;
+  const int64_t begin = int64_t(shared_tile) * p.chunks, end = begin + p.chunks;
   // the walker that had the tile's first chunk, and the one behind its last
   const int64_t w0 = ((begin + 1) * p.walkers - 1) / all, w1 = (end * p.walkers - 1) / all + 1;
   const int64_t from_w = w0 + (w1 - w0) * slice / SLICES, to_w = w0 + (w1 - w0) * (slice + 1) / SLICES;
@@ -557,7 +568,8 @@ __global__ void __launch_bounds__(256 * SLICES) sum_parts_kernel(const SumParts 
     float v[kTogether][8];
 #pragma unroll
     for (int k = 0; k < kTogether; ++k) {
-      const float* from = p.partial + ((w + k + shared_tile) * kCtas + r0 / kTileM) * (BN * kTileM) + (c0 + warp * 8) * kTileM + r0 % kTileM + lane;
+      const float* from = p.partial + ((w + k + shared_tile) * kCtas + r0 / kTileM) * (BN * kTileM) + (c0 + warp * 8) * kTileM +
+                          r0 % kTileM + lane;
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[k][i] = w + k < to_w ? __ldg(from + i * kTileM) : 0.f;
     }

@@ -11,6 +11,8 @@
 // group, head), so no two of them share a word or a bank, and what a hub's bucket costs is what any costs.  The sums
 // of a CTA's warps and then of the CTAs are added in a fixed order: no atomics, the same bits every time.  Both directions are bound by the
 // ids and the rows of bias; the forward keeps the buckets, 2 bytes an edge in the place of the 16 of two ids.
+// us, 18.2 M edges x 8 heads, 870,001 positions: forward 230 (910 MB; without positions 151: two random reads an edge keep the L1 76 %
+// busy), backward 130 and 9 for the last sums (620 MB); 526,450 edges 8.5, 8.4 and 4.5.
 #include "tgt_common.cuh"
 
 namespace tgt {

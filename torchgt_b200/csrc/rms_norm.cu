@@ -6,11 +6,14 @@
 //
 // All of it in fp32, rounded once where it is stored; y comes from v before v is rounded for the residual stream.  In bf16 the
 // forward can leave the next 8 bits of v beside the rounded sum for the backward: with the sum alone its rounding is in dw next
-// to dw's own (2.4e-3 from 64 bits in the 2-norm, with them 1.7e-3), for an eighth more bytes.  What is read and written bounds it: x and the residual in, y and the sum out; dy, the
-// residual stream's gradient and the sum in, dx out.  A row is held in registers between its sums and its results: by a group
-// of 8 to 32 lanes, or by a CTA where it is longer than a warp should hold.  Rows that are a whole number of 16-byte pieces
-// from 16-byte boundaries on move in such pieces, all others value by value.  The weight's gradient is summed per thread over
-// the rows it walks, then over a CTA's groups and over the CTAs in a fixed order: no atomics, the same bits every time.
+// to dw's own (2.4e-3 from 64 bits in the 2-norm, with them 1.7e-3), for an eighth more bytes.
+// What is read and written bounds it: x and the residual in, y and the sum out; dy, the residual stream's gradient and the sum
+// in, dx out.  A row is held in registers between its sums and its results: by a group of 8 to 32 lanes, or by a CTA where it
+// is longer than a warp should hold, the next row on its way meanwhile.  Rows that are a whole number of 16-byte pieces from
+// 16-byte boundaries on move in such pieces, all others value by value.  The weight's gradient is summed per thread over the rows it
+// walks, then over a CTA's groups and over the CTAs in a fixed order: no atomics, the same bits every time.
+// us (a copy's rate would be): bf16 with a residual, 16,384 x 2,048 forward with the kept bits 46 (47), backward 59 (47); 16,384 x
+// 5,120 to e4m3 96 (91); fp32 64,001 x 64 9.8 (10.1) and 11.3 (10.1, in part from the L2).
 #include <cuda_fp8.h>
 
 #include <atomic>
@@ -551,8 +554,8 @@ int forward(const void* x, const void* residual, const void* weight, float eps, 
 }
 
 template <typename T>
-int backward(const void* dy, const void* dsum, const void* v, const int8_t* rest, const void* weight, const float* rstd, int64_t rows, int hidden,
-             void* dx, void* dweight, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+int backward(const void* dy, const void* dsum, const void* v, const int8_t* rest, const void* weight, const float* rstd,
+             int64_t rows, int hidden, void* dx, void* dweight, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
   RmsBwd<T> p{static_cast<const T*>(dy), static_cast<const T*>(dsum), static_cast<const T*>(v), rest,
               static_cast<const T*>(weight), rstd, static_cast<T*>(dx), nullptr, rows, hidden};
   return whole_pieces<T>(hidden, {dy, dsum, v, rest, weight, dx})

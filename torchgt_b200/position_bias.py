@@ -6,8 +6,9 @@
 
 Buckets of one direction, ``n`` of them: distances below ``n // 2`` have a bucket each; the others' borders are even steps of
 the logarithm from there to ``max_distance``, and the last bucket takes everything from its border on.  With ``bidirectional``
-the table's second half is for sources behind their destination (offset > 0); without it those count as distance 0.  The borders are whole numbers,
-``d ** steps >= max_distance ** j * exact ** (steps - j)``, so no rounding of a logarithm decides about a distance."""
+the table's second half is for sources behind their destination (offset > 0); without it those count as distance 0.  The
+borders are whole numbers, ``d ** steps >= max_distance ** j * exact ** (steps - j)``, so no rounding of a logarithm decides
+about a distance."""
 from __future__ import annotations
 
 import functools
@@ -45,7 +46,8 @@ def bucket_borders(num_buckets: int, max_distance: int, bidirectional: bool) -> 
 
 
 def _as_operations(table, edge_index, positions, borders, bidirectional):
-    """The same from operations that a tracer or compiler can record; an id outside the positions is torch's error."""
+    """The same from operations that tracers, compilers and ``torch.func`` can record; an id outside the positions is torch's
+    error."""
     source, destination = edge_index.long().unbind(0)
     if positions is not None:
         source, destination = positions.long()[source], positions.long()[destination]
@@ -81,7 +83,7 @@ def edge_position_bias(table: torch.Tensor, edge_index: torch.Tensor, positions:
     if positions is not None and positions.dim() != 1:
         raise ValueError("positions must be [N]")
     borders = bucket_borders(table.shape[0], max_distance, bool(bidirectional))
-    if not plain_call(*tensors):
+    if not plain_call(*tensors) or not _cabi.native().edge_position_bias_covers(table, edge_index, positions):
         return _as_operations(table, edge_index, positions, borders, bidirectional)
     return _cabi.native().edge_position_bias(table, edge_index, positions, borders, bool(bidirectional))
 
