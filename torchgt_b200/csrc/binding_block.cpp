@@ -5,6 +5,7 @@
 
 #include <ATen/TensorSubclassLikeUtils.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -24,9 +25,13 @@ bool plain(const at::Tensor& t, const at::Device& device, at::ScalarType type) {
 bool kernel_type(at::ScalarType type) { return type == at::kFloat || type == at::kBFloat16; }
 int type_code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? TGT_F32 : TGT_BF16; }
 
-at::Tensor scratch_of(size_t bytes, const at::Tensor& like) {
-  return at::empty({int64_t(bytes < 16 ? 16 : bytes)}, like.options().dtype(at::kByte));
+// An uninitialised tensor next to `like`, straight from the allocator's function: the small calls are bound by the host, and on its
+// way through the dispatcher at::empty takes twice the time.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
 }
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor& like) { return fresh(sizes, like.scalar_type(), like); }
+at::Tensor scratch_of(size_t bytes, const at::Tensor& like) { return fresh({int64_t(bytes < 16 ? 16 : bytes)}, at::kByte, like); }
 
 // ---- root-mean-square norm, with the residual addition in front of it -----------------------------------------------
 // Outputs: the normalised rows and, with a residual, x + residual.
@@ -66,7 +71,7 @@ struct RmsNormRowsBackward : public torch::autograd::Node {
     const at::Tensor dy = grads[0].contiguous(), vc = v.contiguous(), wc = w.contiguous();
     const at::Tensor dsum = ds.defined() ? ds.contiguous() : ds;
     const int64_t hidden = w.numel(), rows = v.numel() / hidden;
-    const at::Tensor dx = at::empty(v.sizes(), dy.options()), dw = at::empty(w.sizes(), dy.options());
+    const at::Tensor dx = fresh(v.sizes(), dy), dw = fresh(w.sizes(), dy);
     size_t bytes = 0;
     check(tgt_rms_norm_bwd_scratch_bytes(rows, int(hidden), type_code(v), &bytes));
     const at::Tensor scratch = scratch_of(bytes, dy);
@@ -91,10 +96,12 @@ bool rms_norm_covers(const at::Tensor& x, const at::Tensor& w, const std::option
   return !residual.has_value() || (plain(*residual, x.device(), x.scalar_type()) && residual->sizes() == x.sizes());
 }
 
-// {norm of x (+ residual), x + residual or nothing}; the sum is left out when nobody wants it
-std::pair<at::Tensor, std::optional<at::Tensor>> add_rms_norm(const at::Tensor& x, const std::optional<at::Tensor>& residual_in,
-                                                              const at::Tensor& w, double eps, bool want_sum) {
-  TORCH_CHECK(rms_norm_covers(x, w, residual_in), "rms_norm: tensors that the kernels do not cover");
+// {norm of x (+ residual), x + residual or nothing}; the sum is left out when nobody wants it.  Nothing, and nothing launched, for
+// tensors that the kernels do not cover.
+std::optional<std::pair<at::Tensor, std::optional<at::Tensor>>> add_rms_norm(const at::Tensor& x,
+                                                                             const std::optional<at::Tensor>& residual_in,
+                                                                             const at::Tensor& w, double eps, bool want_sum) {
+  if (!rms_norm_covers(x, w, residual_in)) return std::nullopt;
   const at::Tensor residual = residual_in.value_or(at::Tensor());
   const c10::cuda::CUDAGuard guard(x.device());
   const bool record = torch::autograd::compute_requires_grad(x, residual, w);
@@ -103,10 +110,10 @@ std::pair<at::Tensor, std::optional<at::Tensor>> add_rms_norm(const at::Tensor& 
   {
     const at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor xc = x.contiguous(), wc = w.contiguous(), rc = residual.defined() ? residual.contiguous() : residual;
-    y = at::empty(x.sizes(), x.options());
-    if (residual.defined() && (want_sum || record)) sum = at::empty(x.sizes(), x.options());
-    if (record && sum.defined() && x.scalar_type() == at::kBFloat16) rest = at::empty(x.sizes(), x.options().dtype(at::kChar));
-    if (record) rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+    y = fresh(x.sizes(), x);
+    if (residual.defined() && (want_sum || record)) sum = fresh(x.sizes(), x);
+    if (record && sum.defined() && x.scalar_type() == at::kBFloat16) rest = fresh(x.sizes(), at::kChar, x);
+    if (record) rstd = fresh({rows}, at::kFloat, x);
     check(tgt_rms_norm_fwd(ptr(xc), ptr(rc), ptr(wc), float(eps), rows, int(hidden), type_code(x), ptr(sum), ptr(rest), ptr(y),
                            record ? fptr(rstd) : nullptr, stream_of(x)));
   }
@@ -126,7 +133,7 @@ std::pair<at::Tensor, std::optional<at::Tensor>> add_rms_norm(const at::Tensor& 
       node->normalised = SavedVariable(x, false);
     }
   }
-  return {y, sum.defined() ? std::optional<at::Tensor>(sum) : std::nullopt};
+  return std::make_pair(y, sum.defined() ? std::optional<at::Tensor>(sum) : std::nullopt);
 }
 
 // {values, scales, x + residual or nothing}; no gradients
@@ -140,10 +147,10 @@ std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>> rms_norm_e4m3(cons
   at::Tensor rc, sum;
   if (residual_in.has_value()) {
     rc = residual_in->contiguous();
-    sum = at::empty(x.sizes(), x.options());
+    sum = fresh(x.sizes(), x);
   }
-  const at::Tensor values = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-  const at::Tensor scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  const at::Tensor values = fresh(x.sizes(), at::kFloat8_e4m3fn, x);
+  const at::Tensor scales = fresh(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
   check(tgt_rms_norm_e4m3(ptr(xc), ptr(rc), ptr(wc), float(eps), rows, int(hidden), type_code(x), ptr(sum), ptr(values),
                           fptr(scales), stream_of(x)));
   return {values, scales, sum.defined() ? std::optional<at::Tensor>(sum) : std::nullopt};
@@ -168,7 +175,7 @@ struct EdgePositionBiasBackward : public torch::autograd::Node {
     }
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(of.device());
-    const at::Tensor d = grads[0].contiguous(), dtable = at::empty({n_buckets, heads}, d.options());
+    const at::Tensor d = grads[0].contiguous(), dtable = fresh({n_buckets, heads}, d);
     size_t bytes = 0;
     check(tgt_edge_position_bias_grad_scratch_bytes(edges, int(n_buckets), int(heads), &bytes));
     const at::Tensor scratch = scratch_of(bytes, d);
@@ -180,19 +187,16 @@ struct EdgePositionBiasBackward : public torch::autograd::Node {
   void release_variables() override { buckets.reset_data(); }
 };
 
-// The caller has checked types and shapes; what is left are wrappers of torch.func, dual numbers and the like.
-bool edge_position_bias_covers(const at::Tensor& table, const at::Tensor& edge_index, const std::optional<at::Tensor>& positions) {
-  auto ids = [&](const at::Tensor& t) { return plain(t, table.device(), at::kLong) || plain(t, table.device(), at::kInt); };
-  return table.defined() && plain(table, table.device(), at::kFloat) && ids(edge_index) && (!positions.has_value() || ids(*positions));
-}
-
-// The caller has checked types, shapes and the borders.
-at::Tensor edge_position_bias(const at::Tensor& table, const at::Tensor& edge_index, const std::optional<at::Tensor>& positions,
+// The caller has checked types, shapes and the borders; nothing, and nothing launched, for what is left: wrappers of torch.func, dual
+// numbers and the like.
+std::optional<at::Tensor> edge_position_bias(const at::Tensor& table, const at::Tensor& edge_index, const std::optional<at::Tensor>& positions,
                               const std::vector<int32_t>& borders, bool both_ways) {
-  TORCH_CHECK(edge_position_bias_covers(table, edge_index, positions) && table.dim() == 2 && edge_index.dim() == 2 &&
-                  edge_index.size(0) == 2 && (!positions.has_value() || positions->dim() == 1) &&
+  auto ids = [&](const at::Tensor& t) { return plain(t, table.device(), at::kLong) || plain(t, table.device(), at::kInt); };
+  if (!table.defined() || !plain(table, table.device(), at::kFloat) || !ids(edge_index) || (positions.has_value() && !ids(*positions)))
+    return std::nullopt;
+  TORCH_CHECK(table.dim() == 2 && edge_index.dim() == 2 && edge_index.size(0) == 2 && (!positions.has_value() || positions->dim() == 1) &&
                   table.size(0) == int64_t(borders.size() + 1) * (both_ways ? 2 : 1),
-              "edge_position_bias: tensors that the kernels do not cover");
+              "edge_position_bias: shapes that do not fit one another");
   const at::Device device = table.device();
   const c10::cuda::CUDAGuard guard(device);
   const int64_t edges = edge_index.size(1), heads = table.size(1);
@@ -202,8 +206,8 @@ at::Tensor edge_position_bias(const at::Tensor& table, const at::Tensor& edge_in
     const at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor tc = table.contiguous(), ec = edge_index.contiguous();
     const at::Tensor pc = positions.has_value() ? positions->contiguous() : at::Tensor();
-    bias = at::empty({edges, heads}, table.options());
-    if (record) buckets = at::empty({edges}, table.options().dtype(at::kShort));
+    bias = fresh({edges, heads}, table);
+    if (record) buckets = fresh({edges}, at::kShort, table);
     // no nodes: every id is outside, which takes a pointer to tell
     const void* where = pc.defined() ? (pc.numel() > 0 ? pc.data_ptr() : static_cast<const void*>(tc.data_ptr())) : nullptr;
     check(tgt_edge_position_bias(ptr(ec), edges, ec.scalar_type() == at::kLong, where, pc.defined() ? pc.numel() : 0,
@@ -284,7 +288,7 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
       const void* from[2];
       void* to[2];
       for (size_t i = 0; i < d.size(); ++i) {
-        dw[i] = at::empty({n, k}, x_.options());
+        dw[i] = fresh({n, k}, x_);
         from[i] = ptr(d[i]);
         to[i] = dw[i].data_ptr();
       }
@@ -297,13 +301,13 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
     if (task_should_compute_output(3)) weight_gradients({dy}, h, out, mid, &result[3]);
     const bool first = task_should_compute_output(1) || task_should_compute_output(2);
     if (!first && !task_should_compute_output(0)) return result;
-    const at::Tensor dg = at::empty_like(g), du = at::empty_like(u);
+    const at::Tensor dg = fresh(g.sizes(), g), du = fresh(u.sizes(), u);
     const at::Tensor wdc = kernel_ready(wd);
     check(tgt_gated_hidden_grad(ptr(dy), ptr(wdc), ptr(g), ptr(u), ptr(l), rows, int(out), int(mid), act, type, ptr(dg), ptr(du), stream));
     if (first) weight_gradients({dg, du}, kernel_ready(x_), mid, in, &result[1]);
     if (task_should_compute_output(0)) {
       const at::Tensor wgc = kernel_ready(wg), wuc = kernel_ready(wu);
-      result[0] = at::empty(x_.sizes(), x_.options());
+      result[0] = fresh(x_.sizes(), x_);
       check(tgt_gated_input_grad(ptr(dg), ptr(du), ptr(wgc), ptr(wuc), rows, int(mid), int(in), type, ptr(result[0]), stream));
     }
     return result;
@@ -334,10 +338,11 @@ bool gated_feed_forward_covers(const at::Tensor& x, const at::Tensor& wg, const 
   return plain(*residual, x.device(), x.scalar_type()) && residual->sizes() == at::IntArrayRef(sizes);
 }
 
-at::Tensor gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
-                              const std::string& activation, const std::optional<at::Tensor>& residual_in) {
+// Nothing, and nothing launched, for tensors that the kernels do not cover.
+std::optional<at::Tensor> gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd,
+                                             const std::string& activation, const std::optional<at::Tensor>& residual_in) {
   const int act = activation_code(activation);
-  TORCH_CHECK(gated_feed_forward_covers(x, wg, wu, wd, residual_in), "gated_feed_forward: tensors that the kernels do not cover");
+  if (!gated_feed_forward_covers(x, wg, wu, wd, residual_in)) return std::nullopt;
   const at::Tensor residual = residual_in.value_or(at::Tensor());
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t in = wg.size(1), mid = wg.size(0), out = wd.size(0), rows = x.numel() / in;
@@ -350,14 +355,14 @@ at::Tensor gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const a
                      rc = residual.defined() ? kernel_ready(residual) : residual;
     auto sizes = x.sizes().vec();
     sizes.back() = mid;
-    h = at::empty(sizes, x.options());
+    h = fresh(sizes, x);
     if (record || type == TGT_F32) {
-      g = at::empty(sizes, x.options());
-      u = at::empty(sizes, x.options());
-      if (type == TGT_BF16) l = at::empty(sizes, x.options());
+      g = fresh(sizes, x);
+      u = fresh(sizes, x);
+      if (type == TGT_BF16) l = fresh(sizes, x);
     }
     sizes.back() = out;
-    y = at::empty(sizes, x.options());
+    y = fresh(sizes, x);
     void* const stream = stream_of(x);
     if (type == TGT_BF16 && !record && few_rows(rows, in, mid)) {
       check(tgt_gated_few_rows(ptr(xc), ptr(wgc), ptr(wuc), ptr(wdc), ptr(rc), rows, int(in), int(mid), int(out), act, ptr(h), ptr(y),
@@ -388,12 +393,9 @@ at::Tensor gated_feed_forward(const at::Tensor& x, const at::Tensor& wg, const a
 }  // namespace
 
 void bind_block(pybind11::module_& m) {
-  m.def("rms_norm_covers", &rms_norm_covers);
   m.def("add_rms_norm", &add_rms_norm, Unlocked());
   m.def("rms_norm_e4m3", &rms_norm_e4m3, Unlocked());
-  m.def("edge_position_bias_covers", &edge_position_bias_covers);
   m.def("edge_position_bias", &edge_position_bias, Unlocked());
-  m.def("gated_feed_forward_covers", &gated_feed_forward_covers);
   m.def("gated_feed_forward", &gated_feed_forward, Unlocked());
 }
 

@@ -34,9 +34,9 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     if residual is not None and residual.shape != x.shape[:-1] + w_down.shape[:1]:
         raise ValueError(f"residual must be {tuple(x.shape[:-1] + w_down.shape[:1])}; got {tuple(residual.shape)}")
     if x.is_cuda and plain_call(x, w_gate, w_up, w_down, residual):
-        native = _cabi.native()
-        if native.gated_feed_forward_covers(x, w_gate, w_up, w_down, residual):
-            return native.gated_feed_forward(x, w_gate, w_up, w_down, activation, residual)
+        y = _cabi.native().gated_feed_forward(x, w_gate, w_up, w_down, activation, residual)
+        if y is not None:
+            return y
     h = _ACTIVATIONS[activation](linear(x, w_gate, None)) * linear(x, w_up, None)
     y = linear(h, w_down, None)
     return y if residual is None else y + residual

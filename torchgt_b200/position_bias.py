@@ -83,9 +83,11 @@ def edge_position_bias(table: torch.Tensor, edge_index: torch.Tensor, positions:
     if positions is not None and positions.dim() != 1:
         raise ValueError("positions must be [N]")
     borders = bucket_borders(table.shape[0], max_distance, bool(bidirectional))
-    if not plain_call(*tensors) or not _cabi.native().edge_position_bias_covers(table, edge_index, positions):
-        return _as_operations(table, edge_index, positions, borders, bidirectional)
-    return _cabi.native().edge_position_bias(table, edge_index, positions, borders, bool(bidirectional))
+    if plain_call(*tensors):
+        bias = _cabi.native().edge_position_bias(table, edge_index, positions, borders, bool(bidirectional))
+        if bias is not None:
+            return bias
+    return _as_operations(table, edge_index, positions, borders, bidirectional)
 
 
 class RelativePositionBias(torch.nn.Module):

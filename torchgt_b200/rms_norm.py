@@ -15,14 +15,16 @@ from .linear import plain_call, unobserved
 
 
 def _eps(x: torch.Tensor, eps: Optional[float]) -> float:
-    """``torch.nn.RMSNorm``'s default."""
-    return torch.finfo(x.dtype).eps if eps is None else eps
+    """``torch.nn.RMSNorm``'s default (of whole numbers any: torch refuses them)."""
+    return eps if eps is not None else torch.finfo(x.dtype).eps if x.is_floating_point() else 0.0
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None) -> torch.Tensor:
     """``x / sqrt(mean(x ** 2) + eps) * weight`` over the last dimension."""
-    if x.is_cuda and weight is not None and plain_call(x, weight) and _cabi.native().rms_norm_covers(x, weight, None):
-        return _cabi.native().add_rms_norm(x, None, weight, _eps(x, eps), False)[0]
+    if x.is_cuda and weight is not None and plain_call(x, weight):
+        out = _cabi.native().add_rms_norm(x, None, weight, _eps(x, eps), False)
+        if out is not None:
+            return out[0]
     return torch.nn.functional.rms_norm(x, (x.shape[-1],), weight, eps)
 
 
@@ -30,9 +32,10 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
                  want_sum: bool = True):
     """``(rms_norm(x + residual), x + residual)`` in one kernel each way.  The norm is that of the sum before it is rounded to
     the tensors' type.  The second is None when ``want_sum`` is false and nothing else needs it."""
-    if (x.is_cuda and weight is not None and plain_call(x, residual, weight) and
-            _cabi.native().rms_norm_covers(x, weight, residual)):
-        return _cabi.native().add_rms_norm(x, residual, weight, _eps(x, eps), want_sum)
+    if x.is_cuda and weight is not None and plain_call(x, residual, weight):
+        out = _cabi.native().add_rms_norm(x, residual, weight, _eps(x, eps), want_sum)
+        if out is not None:
+            return out
     x = x + residual
     return rms_norm(x, weight, eps), x
 
