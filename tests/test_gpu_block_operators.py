@@ -174,3 +174,47 @@ def test_traced_transformed_and_compiled_calls_are_operations():
     assert torch.equal(torch.jit.trace(lambda t: edge_position_bias(t, edges), (tables[0],), check_trace=False)(tables[0]), want[0])
     value, tangent = torch.func.jvp(lambda t: edge_position_bias(t, edges), (tables[0],), (tables[1],))
     assert torch.equal(value, want[0]) and torch.equal(tangent, want[1])
+
+
+def test_two_threads_on_streams_of_their_own():
+    """Calls of every operator from two threads at once, each on its stream and with its sizes, give what they give alone."""
+    import threading
+
+    from torchgt_b200 import edge_position_bias, gated_feed_forward
+    from torchgt_b200.rms_norm import add_rms_norm, rms_norm_quantized
+
+    def work(seed, rows, dtype):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        draw = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dtype)   # noqa: E731
+        x, r, dy = draw(rows, 192), draw(rows, 192), draw(rows, 192)
+        w, wg, wu, wd = draw(192), draw(256, 192) / 14, draw(256, 192) / 14, draw(192, 256) / 16
+        table = torch.randn(32, HEADS, generator=gen, device="cuda", requires_grad=True)
+        edges = torch.randint(0, rows, (2, 6 * rows), generator=gen, device="cuda")
+        dbias = torch.randn(6 * rows, HEADS, generator=gen, device="cuda")
+
+        def step():
+            leaves = [t.detach().requires_grad_() for t in (x, r, w, wg, wu, wd)]
+            y, total = add_rms_norm(*leaves[:3], EPS)
+            y = gated_feed_forward(y, *leaves[3:], "silu", total)
+            with torch.no_grad():
+                values, scales, _ = rms_norm_quantized(x, w, EPS, r)
+                few = gated_feed_forward(x[:7], wg, wu, wd)
+            return [y.detach(), *torch.autograd.grad(y, leaves, dy), values.view(torch.uint8), scales, few,
+                    *torch.autograd.grad(edge_position_bias(table, edges), [table], dbias)]
+        return step
+    steps = [work(1, 1500, torch.bfloat16), work(2, 5000, torch.bfloat16), work(3, 3000, torch.float32)]
+    wanted = [step() for step in steps]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(step, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                if not all(torch.equal(a, b) for a, b in zip(step(), want)):
+                    wrong.append(step)
+    threads = [threading.Thread(target=run, args=pair) for pair in zip(steps, wanted)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not wrong and not any(t.is_alive() for t in threads)

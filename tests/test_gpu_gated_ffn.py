@@ -121,6 +121,27 @@ def test_a_few_rows_without_gradients(rows, act):
         assert torch.equal(gated_feed_forward(x[:1], wg, wu, wd, act, r[:1]), got[:1]) or rows > 8
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("rows,n_in,n_mid,n_out", [(33, 2048, 512, 64), (40, 4096, 72, 768), (100, 520, 5632, 200), (129, 1096, 2056, 72),
+                                                   (333, 768, 2048, 768), (500, 4104, 264, 136), (700, 64, 4096, 8)])
+def test_tiles_split_along_k(rows, n_in, n_mid, n_out, act):
+    """Products with fewer tiles than the chip has SMs, some of them several CTAs to a tile; with and without what gradients keep."""
+    from torchgt_b200 import gated_feed_forward
+    x, wg, wu, wd, r, _ = _inputs(rows, n_in, n_mid, n_out, torch.bfloat16, 29)
+    for residual in (None, r):
+        want = _formula(x, wg, wu, wd, act, residual, None)["y"]
+        with torch.no_grad():
+            got = gated_feed_forward(x, wg, wu, wd, act, residual)
+        _within(got, want, "y")
+        kept = gated_feed_forward(x.clone().requires_grad_(), wg, wu, wd, act, residual)
+        assert torch.equal(got, kept.detach())
+    x[3] = float("nan")
+    with torch.no_grad():
+        spoilt = gated_feed_forward(x, wg, wu, wd, act, r)
+    others = [i for i in range(rows) if i != 3]
+    assert torch.equal(spoilt[others], got[others]) and bool(spoilt[3].isnan().all())
+
+
 @pytest.mark.parametrize("rows,n_in,n_mid,n_out", [(1, 64, 64, 64), (3, 64, 128, 4), (200, 128, 64, 100), (4097, 64, 128, 64), (9000, 64, 64, 64),
                                                    (700, 1024, 1024, 1024)])
 def test_fp32(rows, n_in, n_mid, n_out):

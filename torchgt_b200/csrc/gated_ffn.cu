@@ -69,28 +69,28 @@ int tiles_of(int64_t n, int tile) { return int((n + tile - 1) / tile); }
     if (_rc != TGT_OK) return _rc;     \
   } while (0)
 
-// How a product is cut up: tiles of 128 rows of a CTA, or of 256 of a pair, x `bn` columns.
+// How a product is cut up: tiles of 128 rows of a CTA, or of 256 of a pair, x `bn` columns; `split` CTAs along k to one of a CTA.
 struct Cut {
   bool pair;
-  int bn;
+  int bn, split;
   int rows() const { return pair ? 2 * gemm::kTileM : gemm::kTileM; }
   int b_rows() const { return pair ? bn / 2 : bn; }      // of B that one copy brings in
 };
 
-template <int BN, bool PAIR, bool A_MN, bool B_MN, gemm::Finish FINISH>
-int launch(const Gemm& p, int walkers, cudaStream_t stream, bool chained = false) {
-  constexpr int kSmem = gemm::smem_bytes(PAIR ? BN / 2 : BN, FINISH);
-  TGT_RETURN_IF(allow_shared_memory<gemm::gemm_kernel<BN, PAIR, A_MN, B_MN, FINISH>>(kSmem));
+template <int BN, bool PAIR, bool A_MN, bool B_MN, gemm::Finish FINISH, int SPLIT = 1>
+int launch(const Gemm& p, int walkers, cudaStream_t stream, bool chained) {
+  constexpr int kSmem = gemm::smem_bytes(PAIR ? BN / 2 : BN, FINISH), kCluster = PAIR ? 2 : SPLIT;
+  TGT_RETURN_IF(allow_shared_memory<gemm::gemm_kernel<BN, PAIR, A_MN, B_MN, FINISH, SPLIT>>(kSmem));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(walkers * (PAIR ? 2 : 1));
+  cfg.gridDim = dim3(walkers * kCluster);
   cfg.blockDim = dim3(gemm::kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  if (PAIR) {
+  if (kCluster > 1) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = 2;
+    attr[cfg.numAttrs].val.clusterDim.x = kCluster;
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
@@ -99,7 +99,7 @@ int launch(const Gemm& p, int walkers, cudaStream_t stream, bool chained = false
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  TGT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm::gemm_kernel<BN, PAIR, A_MN, B_MN, FINISH>, p));
+  TGT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm::gemm_kernel<BN, PAIR, A_MN, B_MN, FINISH, SPLIT>, p));
   return TGT_OK;
 }
 
@@ -115,13 +115,18 @@ struct Plan {
   }
 };
 
-constexpr Cut kCuts[] = {{true, 256}, {true, 128}, {false, 256}, {false, 128}, {false, 64}};
+constexpr Cut kCuts[] = {{true, 256, 1}, {true, 128, 1}, {false, 256, 1}, {false, 128, 1}, {false, 64, 1}};
+enum Along { kWhole, kShare, kSplit };      // what may be done along k with too few tiles
+
 // The cut, and whether the last round's tiles are shared, of the least time by what was measured: us a chunk of k, a finish of
 // 256 columns, a start, and sharing.  us by pairs of 256 and 128 columns, single CTAs of 256, 128 and 64: y of 8,191 rows, 5,632 x 2,048
 // 137, 153, 187, 172, 307; 333 rows, 2,048 x 768 16.6, 12.6, 16.3, 13.7, 11.8; dx of 64,000 rows, 128 x 64 12.8, 11.9, 13.3, 10.0, 8.5;
 // h of 1,000 rows, 768 x 2,048, with what is kept 12.5, 14.6, 11.5, 13.0, -.  Shared or not: two weight gradients of 16,384 rows, 2,816 x
-// 1,024 135 / 166 (88 tiles for 74 pairs), of 64,000 rows, 128 x 64 19 / 223; one of 16,384 rows, 1,024 x 2,816 (44 tiles) 89 / 83.
-Plan plan_for(int products, int64_t m, int columns, int narrowest, int chunks, double finish, bool may_share) {
+// 1,024 135 / 166 (88 tiles for 74 pairs), of 64,000 rows, 128 x 64 19 / 223; one of 16,384 rows, 1,024 x 2,816 (44 tiles) 89 / 83.  By one
+// CTA a tile, 2, 4 and 8: y of 40 rows, 2,048 x 768 11.0, 8.7, 7.5, 6.9; of 333 rows 11.4, 9.5; of 100 rows, 5,632 x 2,048 23.7, 15.6, 12.1;
+// h of 40 rows, 768 x 2,048 6.8, 7.9, 9.0.
+Plan plan_for(int products, int64_t m, int columns, int narrowest, int chunks, double finish, Along along) {
+  const bool may_share = along == kShare;
   constexpr double kChunkTime[] = {0.39, 0.255, 0.42, 0.277, 0.235}, kStart[] = {1, 1, 0, 0, 0};
   Plan best{};
   double least = 0;
@@ -152,6 +157,19 @@ Plan plan_for(int products, int64_t m, int columns, int narrowest, int chunks, d
         least = time;
       }
     }
+    // Several CTAs a tile where there are SMs for them: what they put together, and that they start and end together, in us.
+    if (along != kSplit || q.cut.pair || q.cut.bn != narrowest) continue;
+    double together = q.cut.bn == 64 ? 2.2 : 2.5;
+    for (int split = 2; split <= 8 && tiles * split <= 128 && chunks >= 2 * split; split *= 2) {
+      together += q.cut.bn == 64 ? 0.25 : 1.4;
+      const double time = (chunks + split - 1) / split * kChunkTime[i] * 0.8 + together;
+      if (time < least) {
+        best = q;
+        best.cut.split = split;
+        best.whole = best.walkers = int(tiles);
+        least = time;
+      }
+    }
   }
   return best;
 }
@@ -163,6 +181,11 @@ int launch_cut(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cuda
       return set_error(TGT_ERR_WORKSPACE, "scratch holds %zu bytes, %zu needed", scratch_bytes, q.scratch());
     TGT_CHECK_ARG(aligned16(scratch), "scratch must be 16-byte aligned");
     p.partial = static_cast<float*>(scratch);
+  }
+  if constexpr (!PAIR && !B_MN && (FINISH == gemm::kGated ? BN == 128 : BN == 64)) {
+    if (q.cut.split == 2) return launch<BN, PAIR, A_MN, B_MN, FINISH, 2>(p, q.walkers, stream, chained);
+    if (q.cut.split == 4) return launch<BN, PAIR, A_MN, B_MN, FINISH, 4>(p, q.walkers, stream, chained);
+    if (q.cut.split == 8) return launch<BN, PAIR, A_MN, B_MN, FINISH, 8>(p, q.walkers, stream, chained);
   }
   TGT_RETURN_IF(launch<BN, PAIR, A_MN, B_MN, FINISH>(p, q.walkers, stream, chained));
   if constexpr (A_MN) {
@@ -192,7 +215,7 @@ int launch_plan(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cud
 // the finishes' times of 256 columns (us)
 constexpr double kPlainTime = 3, kPlusTime = 4, kGatedTime = 3, kKeptTime = 4, kGradTime = 5;
 Plan weight_grad_plan(int count, int64_t rows, int out_features, int in_features) {
-  return plan_for(count, out_features, in_features, 64, tiles_of(rows, gemm::kChunk), kPlainTime, true);
+  return plan_for(count, out_features, in_features, 64, tiles_of(rows, gemm::kChunk), kPlainTime, kShare);
 }
 
 int check_widths(int64_t rows, int a, int b, int dtype, int act) {
@@ -265,7 +288,7 @@ extern "C" int tgt_gated_hidden(const void* x, const void* w_gate, const void* w
   }
   Gemm p{};
   TGT_RETURN_IF(expired_wait_word(&p.expired));
-  const Plan q = plan_for(1, rows, 2 * mid, 128, tiles_of(in, gemm::kChunk), gate != nullptr ? kKeptTime : kGatedTime, false);
+  const Plan q = plan_for(1, rows, 2 * mid, 128, tiles_of(in, gemm::kChunk), gate != nullptr ? kKeptTime : kGatedTime, kSplit);
   TGT_RETURN_IF(operand(&p.a[0], x, rows, in, false, gemm::kTileM));
   TGT_RETURN_IF(operand(&p.b[0], w_gate, mid, in, false, q.cut.bn / 2));
   TGT_RETURN_IF(operand(&p.b[1], w_up, mid, in, false, q.cut.bn / 2));
@@ -296,7 +319,7 @@ int gated_output(const void* h, const void* w_down, const void* add, int64_t row
   }
   Gemm p{};
   TGT_RETURN_IF(expired_wait_word(&p.expired));
-  const Plan q = plan_for(1, rows, out, 64, tiles_of(mid, gemm::kChunk), add != nullptr ? kPlusTime : kPlainTime, false);
+  const Plan q = plan_for(1, rows, out, 64, tiles_of(mid, gemm::kChunk), add != nullptr ? kPlusTime : kPlainTime, kSplit);
   TGT_RETURN_IF(operand(&p.a[0], h, rows, mid, false, gemm::kTileM));
   TGT_RETURN_IF(operand(&p.b[0], w_down, out, mid, false, q.cut.b_rows()));
   p.a[1] = p.a[0]; p.b[1] = p.b[0];
@@ -351,7 +374,7 @@ extern "C" int tgt_gated_hidden_grad(const void* dy, const void* w_down, const v
   }
   Gemm p{};
   TGT_RETURN_IF(expired_wait_word(&p.expired));
-  const Plan q = plan_for(1, rows, mid, 64, tiles_of(out, gemm::kChunk), kGradTime, false);
+  const Plan q = plan_for(1, rows, mid, 64, tiles_of(out, gemm::kChunk), kGradTime, kWhole);
   TGT_RETURN_IF(operand(&p.a[0], dy, rows, out, false, gemm::kTileM));
   TGT_RETURN_IF(operand(&p.b[0], w_down, out, mid, true, q.cut.b_rows()));
   p.a[1] = p.a[0]; p.b[1] = p.b[0];
@@ -380,7 +403,7 @@ extern "C" int tgt_gated_input_grad(const void* dgate, const void* dup, const vo
   }
   Gemm p{};
   TGT_RETURN_IF(expired_wait_word(&p.expired));
-  const Plan q = plan_for(1, rows, in, 64, 2 * tiles_of(mid, gemm::kChunk), kPlainTime, false);
+  const Plan q = plan_for(1, rows, in, 64, 2 * tiles_of(mid, gemm::kChunk), kPlainTime, kWhole);
   TGT_RETURN_IF(operand(&p.a[0], dgate, rows, mid, false, gemm::kTileM));
   TGT_RETURN_IF(operand(&p.a[1], dup, rows, mid, false, gemm::kTileM));
   TGT_RETURN_IF(operand(&p.b[0], w_gate, mid, in, true, q.cut.b_rows()));

@@ -4,7 +4,8 @@
 //
 //   D[m][n] = sum over k of A[m][k] B[n][k]
 //
-// A CTA takes tiles of 128 x BN, or two CTAs (PAIR) tiles of 256 x BN together: each has 128 rows of A and of the sums and
+// A CTA takes tiles of 128 x BN; or several (SPLIT) take one between them, each a part of k, and each finishes a part of the rows from
+// all their sums, which they read from one another's shared memory; or two CTAs (PAIR) tiles of 256 x BN together: each has 128 rows of A and of the sums and
 // brings in half of B's rows, and the first issues the products for both, so a tile costs a third less of what the L2 hands
 // out.  One warp brings the operands in by TMA, 64 of k at a time, into a ring of stages; one issues tcgen05.mma on them,
 // four a stage; eight finish the tile before from the other half of the tensor memory: 32 rows and half of the columns
@@ -115,8 +116,21 @@ __device__ __forceinline__ uint32_t first_ctas(uint32_t address) {
   if constexpr (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(address) : "r"(address));
   return address;
 }
-__device__ __forceinline__ void pair_barrier() {                 // every thread of both CTAs
+__device__ __forceinline__ void cluster_barrier() {              // every thread of all CTAs
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// 16 bytes of shared memory of CTA `cta` of the cluster, at the place that `address` is in this one's
+__device__ __forceinline__ float4 load_of(uint32_t address, int cta) {
+  float4 v;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address), "r"(cta) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t word_of(uint32_t address, int cta) {
+  uint32_t v;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
+               : "=r"(v) : "r"(address), "r"(cta) : "memory");
+  return v;
 }
 template <bool PAIR>
 __device__ __forceinline__ void load(uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -132,7 +146,8 @@ __device__ __forceinline__ void load(uint32_t to, const CUtensorMap* map, int x,
 }
 
 // The tiles of a walker (a CTA, or a pair of them), in the order all its warps take them: whole ones round by round, then its
-// share of the chunks of the others, which is a part of a tile or of several.
+// share of the chunks of the others, which is a part of a tile or of several.  With SPLIT the CTA's part of the one tile of its cluster.
+template <int SPLIT>
 struct Work {
   int64_t at, end;             // of the shared chunks
   int next_tile, whole, step, chunks, tile, k0, k1;
@@ -146,8 +161,8 @@ struct Work {
     if (next_tile < whole) {
       tile = next_tile;
       next_tile += step;
-      k0 = 0;
-      k1 = chunks;
+      k0 = SPLIT == 1 ? 0 : int(int64_t(chunks) * (blockIdx.x % SPLIT) / SPLIT);
+      k1 = SPLIT == 1 ? chunks : int(int64_t(chunks) * (blockIdx.x % SPLIT + 1) / SPLIT);
       return true;
     }
     if (at >= end) return false;
@@ -207,10 +222,11 @@ __device__ __forceinline__ float whole(uint32_t upper, uint32_t lower, int i, in
   return __uint_as_float(__byte_perm(lower, upper, i == 0 ? (which == 0 ? 0x5400 : 0x5411) : (which == 0 ? 0x7622 : 0x7633)));
 }
 
-template <int BN, bool PAIR, bool A_MN, bool B_MN, Finish FINISH>
+template <int BN, bool PAIR, bool A_MN, bool B_MN, Finish FINISH, int SPLIT = 1>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Gemm p) {
   constexpr int kRowsB = PAIR ? BN / 2 : BN, kStages = stages_of(kRowsB, FINISH), kStage = stage_bytes(kRowsB);
   constexpr int kCtas = PAIR ? 2 : 1, kTileRows = kTileM * kCtas;
+  static_assert(SPLIT == 1 || (!PAIR && FINISH != kGatedGrad && kStages * kStage >= kTileM * BN * 4), "sums in the place of the ring");
   constexpr bool kShares = A_MN && FINISH == kPlain;     // weight gradients: few tiles, long sums
   extern __shared__ uint8_t s_raw[];
   const uint32_t s_ring = (tc::smem_address(s_raw) + 1023) & ~1023u;
@@ -220,10 +236,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   uint64_t* const s_sums = s_empty + kStages;            // two: the sums of a half are complete
   uint64_t* const s_taken = s_sums + 2;                  // two: the sums of a half have been read; of a pair the first CTA's
   uint64_t* const s_drained = s_taken + 2;
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_drained + 1);
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_drained + 1);     // and, next to it, whether a wait of a split tile ran out
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = PAIR ? blockIdx.x % 2 : 0;            // in the pair: clusters of two along x
-  const int walker = blockIdx.x / kCtas;
+  const int walker = blockIdx.x / (kCtas * SPLIT);
 
   if (warp == kFinishWarps && lane == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -239,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       tma::barrier_init(s_taken + i, kFinishWarps * kCtas);
     }
     tma::barrier_init(s_drained, 1);
+    s_tmem[1] = 0u;
     tma::barriers_ready();
   }
   __syncwarp();
@@ -246,11 +263,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   if (warp == kFinishWarps + 1) allocate<PAIR, 2 * BN>(s_tmem);
   tc::fence_before_barrier();
   __syncthreads();
-  if constexpr (PAIR) pair_barrier();
+  if constexpr (PAIR) cluster_barrier();
   tc::fence_after_barrier();
   const uint32_t tmem = *s_tmem;
   dependent_wait();                                      // for h; before any wait here that has a limit
-  Work work(p, walker, gridDim.x / kCtas);
+  Work<SPLIT> work(p, walker, gridDim.x / (kCtas * SPLIT));
 
   // The two warps that feed the tensor cores go through their loops together and elect a lane where something is issued: in code that a
   // lane runs alone the compiler cannot keep what an instruction takes in uniform registers (tiles of 128 x 128 and 128 x 64
@@ -397,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     // What the finish reads of global memory comes by asynchronous copies into places of the lane's own, a piece of 8 columns
     // of every matrix at a time: as soon as a piece has been read its place is filled with the piece of the next 32 columns, or of
     // the next tile.  (As loads into registers they were waited for a piece at a time: dgate and dup of 16,384 x 2,816 152 us.)
-    constexpr int kRead = read_by(FINISH);
+    constexpr int kRead = SPLIT == 1 ? read_by(FINISH) : 0;
     const uint32_t s_read = tc::smem_address(s_block + kBlockBytes + lane * 16);
     auto fetch = [&](int i, int row0, int col0) {
       const int r = row0 + first + 8 * i, col = col0 + 8 * piece;
@@ -415,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
       for (int k = 0; k < kRead; ++k) v[k] = *reinterpret_cast<const uint4*>(s_block + kBlockBytes + lane * 16 + (k * 4 + i) * 512);
     };
-    Work ahead = work;                           // a step in front of `work`: what is fetched
+    Work<SPLIT> ahead = work;                           // a step in front of `work`: what is fetched
     int ahead_row = 0, ahead_col = 0, ahead_j = kCols;
     auto advance = [&]() {
       ahead_j += 64;
@@ -445,8 +462,22 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       if (ok && !(ok = tc::wait(s_sums + half, complete)) && lane == 0) tc::report_expired_wait(p.expired);
       ok = __all_sync(~0u, ok);
       tc::fence_after_barrier();
+      if constexpr (SPLIT > 1) {
+        // in the place of the ring, which has been used up: rows of BN sums, their 16-byte pieces in an order by row
 #pragma unroll 1
-      for (int j = side * 32; j < kCols; j += 64) {
+        for (int j = side * 32; j < BN; j += 64) {
+          float v[32];
+          sums(from + j, v);
+          uint8_t* const to = s_raw + (s_ring - tc::smem_address(s_raw)) + (rows0 + lane) * (BN * 4);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(to + ((j / 4 + i) ^ (lane & 7)) * 16) =
+                make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+        if (!ok && lane == 0) s_tmem[1] = 1u;            // copies that come late may write there still
+      }
+#pragma unroll 1
+      for (int j = SPLIT == 1 ? side * 32 : kCols; j < kCols; j += 64) {
         const int col = col0 + j;
         float v[32];
         sums(from + j, v);
@@ -539,7 +570,60 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   __syncwarp();
   tc::fence_before_barrier();
   __syncthreads();
-  if constexpr (PAIR) pair_barrier();                    // neither uses the other's shared or tensor memory any more
+  if constexpr (SPLIT > 1) {
+    cluster_barrier();                                   // all parts' sums are in place
+    constexpr int kCols = FINISH == kGated ? BN / 2 : BN, kPieces = kCols / 8, kRows = kTileM / SPLIT;
+    int m_tile, n_tile;
+    place(p.m_tiles, p.n_tiles, walker, m_tile, n_tile);
+    bool failed = false;
+#pragma unroll
+    for (int k = 0; k < SPLIT; ++k) failed |= word_of(tc::smem_address(s_tmem + 1), k) != 0u;
+    // 8 columns from `column` on of row r of the tile, summed over the parts in their order
+    auto all_parts = [&](int r, int column, float (&v)[8]) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < SPLIT; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 f = load_of(s_ring + r * (BN * 4) + ((column / 4 + i) ^ (r & 7)) * 16, k);
+          v[4 * i] += f.x; v[4 * i + 1] += f.y; v[4 * i + 2] += f.z; v[4 * i + 3] += f.w;
+        }
+      if (failed) v[0] = v[1] = v[2] = v[3] = v[4] = v[5] = v[6] = v[7] = __int_as_float(0x7fffffff);
+    };
+    for (int t = threadIdx.x; t < kRows * kPieces; t += kThreads) {
+      const int r = blockIdx.x % SPLIT * kRows + t / kPieces, c = t % kPieces * 8;
+      const int64_t row = int64_t(m_tile) * kTileM + r;
+      const int col = n_tile * kCols + c;
+      if (row >= p.m || col >= p.n) continue;
+      const int64_t at = row * p.n + col;
+      float v[8];
+      all_parts(r, c, v);
+      auto store = [&](uint16_t* to, auto&& word) { *reinterpret_cast<uint4*>(to + at) = make_uint4(word(0), word(2), word(4), word(6)); };
+      if constexpr (FINISH == kGated) {
+        float u[8];
+        all_parts(r, BN / 2 + c, u);
+        if (p.keep) {
+          store(p.out[1], [&](int i) { return upper_pair(v[i], v[i + 1]); });
+          store(p.out[2], [&](int i) { return upper_pair(u[i], u[i + 1]); });
+          store(p.out[3], [&](int i) { return lower_pair(v[i], u[i], v[i + 1], u[i + 1]); });
+        }
+        with_activation(p.act, [&](auto act) {
+          float unused;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = activate<decltype(act)::value, false>(v[i], unused) * u[i];
+        });
+      } else if constexpr (FINISH == kPlus) {
+        float f[8];
+        Lane<__nv_bfloat16, 16>::load(reinterpret_cast<const __nv_bfloat16*>(p.read[0]) + at, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += f[i];
+      }
+      store(p.out[0], [&](int i) { return f32_to_bf16x2(v[i], v[i + 1]); });
+    }
+    cluster_barrier();                                   // nobody reads another's sums any more
+  }
+  if constexpr (PAIR) cluster_barrier();                 // neither uses the other's shared or tensor memory any more
   if (warp == kFinishWarps + 1) release<PAIR, 2 * BN>(tmem);
 }
 
