@@ -157,10 +157,12 @@ Plan plan_for(int products, int64_t m, int columns, int narrowest, int chunks, d
         least = time;
       }
     }
-    // Several CTAs a tile where there are SMs for them: what they put together, and that they start and end together, in us.
+    // Several CTAs a tile where there are SMs for them (clusters of two find all, larger ones not): what they put together, and that
+    // they start and end together, in us.
     if (along != kSplit || q.cut.pair || q.cut.bn != narrowest) continue;
     double together = q.cut.bn == 64 ? 2.2 : 2.5;
-    for (int split = 2; split <= 8 && tiles * split <= 128 && chunks >= 2 * split; split *= 2) {
+    for (int split = 2; split <= 8 && tiles * split <= (split == 2 ? sm_count() : sm_count() * 7 / 8) && chunks >= 2 * split;
+         split *= 2) {
       together += q.cut.bn == 64 ? 0.25 : 1.4;
       const double time = (chunks + split - 1) / split * kChunkTime[i] * 0.8 + together;
       if (time < least) {
