@@ -159,7 +159,7 @@ Plan plan_for(int products, int64_t m, int columns, int narrowest, int chunks, d
     }
     // Several CTAs a tile where there are SMs for them (clusters of two find all, larger ones not): what they put together, and that
     // they start and end together, in us.
-    if (along != kSplit || q.cut.pair || q.cut.bn != narrowest) continue;
+    if (along != kSplit || q.cut.pair || q.cut.bn > 128) continue;
     double together = q.cut.bn == 64 ? 2.2 : 2.5;
     for (int split = 2; split <= 8 && tiles * split <= (split == 2 ? sm_count() : sm_count() * 7 / 8) && chunks >= 2 * split;
          split *= 2) {
@@ -184,7 +184,7 @@ int launch_cut(const Plan& q, Gemm& p, void* scratch, size_t scratch_bytes, cuda
     TGT_CHECK_ARG(aligned16(scratch), "scratch must be 16-byte aligned");
     p.partial = static_cast<float*>(scratch);
   }
-  if constexpr (!PAIR && !B_MN && (FINISH == gemm::kGated ? BN == 128 : BN == 64)) {
+  if constexpr (!PAIR && !B_MN && BN <= 128) {
     if (q.cut.split == 2) return launch<BN, PAIR, A_MN, B_MN, FINISH, 2>(p, q.walkers, stream, chained);
     if (q.cut.split == 4) return launch<BN, PAIR, A_MN, B_MN, FINISH, 4>(p, q.walkers, stream, chained);
     if (q.cut.split == 8) return launch<BN, PAIR, A_MN, B_MN, FINISH, 8>(p, q.walkers, stream, chained);
