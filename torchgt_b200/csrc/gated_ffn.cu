@@ -123,8 +123,9 @@ enum Along { kWhole, kShare, kSplit };      // what may be done along k with too
 // 137, 153, 187, 172, 307; 333 rows, 2,048 x 768 16.6, 12.6, 16.3, 13.7, 11.8; dx of 64,000 rows, 128 x 64 12.8, 11.9, 13.3, 10.0, 8.5;
 // h of 1,000 rows, 768 x 2,048, with what is kept 12.5, 14.6, 11.5, 13.0, -.  Shared or not: two weight gradients of 16,384 rows, 2,816 x
 // 1,024 135 / 166 (88 tiles for 74 pairs), of 64,000 rows, 128 x 64 19 / 223; one of 16,384 rows, 1,024 x 2,816 (44 tiles) 89 / 83.  By one
-// CTA a tile, 2, 4 and 8: y of 40 rows, 2,048 x 768 11.0, 8.7, 7.5, 6.9; of 333 rows 11.4, 9.5; of 100 rows, 5,632 x 2,048 23.7, 15.6, 12.1;
-// h of 40 rows, 768 x 2,048 6.8, 7.9, 9.0.
+// CTA a tile, 2, 4 and 8 of 64 columns: y of 40 rows, 2,048 x 768 11.0, 8.7, 7.5, 6.9; of 333 rows 11.4, 9.5; of 100 rows, 5,632 x 2,048
+// 23.7, 15.6, 12.1; h of 40 rows, 768 x 2,048 6.8, 7.9, 9.0.  By one, and 2 of 128 columns: y of 333 rows, 5,632 x 2,048 25.1, 18.7; of
+// 600 rows, 4,096 x 1,024 19.1, 15.5.
 Plan plan_for(int products, int64_t m, int columns, int narrowest, int chunks, double finish, Along along) {
   const bool may_share = along == kShare;
   constexpr double kChunkTime[] = {0.39, 0.255, 0.42, 0.277, 0.235}, kStart[] = {1, 1, 0, 0, 0};

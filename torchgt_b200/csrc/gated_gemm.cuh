@@ -4,10 +4,10 @@
 //
 //   D[m][n] = sum over k of A[m][k] B[n][k]
 //
-// A CTA takes tiles of 128 x BN; or several (SPLIT) take one between them, each a part of k, and each finishes a part of the rows from
-// all their sums, which they read from one another's shared memory; or two CTAs (PAIR) tiles of 256 x BN together: each has 128 rows of A and of the sums and
-// brings in half of B's rows, and the first issues the products for both, so a tile costs a third less of what the L2 hands
-// out.  One warp brings the operands in by TMA, 64 of k at a time, into a ring of stages; one issues tcgen05.mma on them,
+// A CTA takes tiles of 128 x BN; or several (SPLIT) take one between them, each a part of k, and each finishes a part of
+// the rows from all their sums, which they read from one another's shared memory; or two CTAs (PAIR) take tiles of 256 x BN
+// together: each has 128 rows of A and of the sums and brings in half of B's rows, and the first issues the products for
+// both, so a tile costs a third less of what the L2 hands out.  One warp brings the operands in by TMA, 64 of k at a time, into a ring of stages; one issues tcgen05.mma on them,
 // four a stage; eight finish the tile before from the other half of the tensor memory: 32 rows and half of the columns
 // each, 32 columns at a time.  A lane reads a row of the sums; what is read and written of global memory goes by four lanes
 // to 64 bytes of a row, and 4 KB of shared memory per warp stand between the two.  An operand is `k`-major (rows of k, as x

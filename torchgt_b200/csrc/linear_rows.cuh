@@ -17,15 +17,15 @@ __device__ __forceinline__ float gelu_slope(float x) {
   return normal_cdf(x) + x * (0.39894228040143267794f * expf(-0.5f * x * x));
 }
 
-// 1 / (1 + exp(-x)) to about 2^-22: the power of two of x log2(e), whose rounding is put back to first order, and the
-// approximate reciprocal (1 unit).  0 below -87, where the quotient leaves the normal numbers, and for whatever a NaN makes of it.
+// 1 / (1 + exp(-x)) to about 2^-22, from the mathematics: exp(-y) = 2^t exp(r) with t = -y log2(e) as it rounds and r = -y - t ln(2)
+// what that leaves, at most 1e-5, so exp(r) is 1 + r; then the approximate reciprocal (1 unit).  0 below -87, where the quotient
+// leaves the normal numbers, and for whatever a NaN makes of it.
 __device__ __forceinline__ float logistic(float x) {
-  constexpr float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299e-8f;      // their sum: log2(e)
   const float y = fminf(fmaxf(x, -87.f), 87.f);
-  const float t = -y * kLog2e, rest = fmaf(-y, kLog2e, -t) - y * kLog2eRest;
+  const float t = -y * 1.44269504088896341f, r = fmaf(-t, 0.693147180559945309f, -y);
   float e, s;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  e = fmaf(e, rest * 0.693147180559945309f, e);
+  e = fmaf(e, r, e);
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
   return x < -87.f ? 0.f : s;
 }
