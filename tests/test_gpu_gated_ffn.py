@@ -121,6 +121,27 @@ def test_a_few_rows_without_gradients(rows, act):
         assert torch.equal(gated_feed_forward(x[:1], wg, wu, wd, act, r[:1]), got[:1]) or rows > 8
 
 
+@pytest.mark.parametrize("rows", [1, 8, 13, 16, 27, 32])
+@pytest.mark.parametrize("n_in,n_mid,n_out", [(264, 11016, 1016), (136, 1800, 2376), (1032, 72, 4096), (64, 4744, 4744), (24, 200, 16392)])
+def test_a_few_rows_of_wide_outputs(rows, n_in, n_mid, n_out):
+    """One set of columns of y a CTA, two, and more CTAs than SMs; more of k than the steps that are under way."""
+    from torchgt_b200 import gated_feed_forward
+    x, wg, wu, wd, r, _ = _inputs(rows, n_in, n_mid, n_out, torch.bfloat16, 31)
+    got = gated_feed_forward(x, wg, wu, wd, "silu", r)
+    _within(got, _formula(x, wg, wu, wd, "silu", r, None)["y"], "y")
+    x[rows - 1] = float("inf")
+    spoilt = gated_feed_forward(x, wg, wu, wd, "silu", r)
+    assert torch.equal(spoilt[:rows - 1], got[:rows - 1]) and not bool(spoilt[rows - 1].isfinite().any())
+    h = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(h):
+        y = gated_feed_forward(x, wg, wu, wd, "silu", r)
+    x[rows - 1] = 0.5
+    want = gated_feed_forward(x, wg, wu, wd, "silu", r)
+    for _ in range(3):
+        h.replay()
+    assert torch.equal(y, want)
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("rows,n_in,n_mid,n_out", [(33, 2048, 512, 64), (40, 4096, 72, 768), (100, 520, 5632, 200), (129, 1096, 2056, 72),
                                                    (333, 768, 2048, 768), (500, 4104, 264, 136), (700, 64, 4096, 8)])

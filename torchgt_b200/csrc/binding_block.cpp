@@ -238,9 +238,11 @@ at::Tensor kernel_ready(const at::Tensor& t) {
 }
 
 // Rows without gradients for which the kernels of gated_rows.cu are ahead of tiles of 128 rows.  us, weights not in the L2: 2,048 x
-// 5,632, one row 18 / 46, 16 rows 23 / 43, 32 rows 32 / 37; 768 x 2,048, 32 rows 10 / 19; 4,096 x 11,008, one row 51 / 102, 16 rows
-// 69 / 80, and at 32 rows tiles.
-bool few_rows(int64_t rows, int64_t in, int64_t mid) { return rows <= 16 || (rows <= 32 && in * mid <= int64_t(1) << 24); }
+// 5,632 x 2,048, one row 14.5 / 35, 16 rows 17 / 29, 32 rows 22 / 24; 768 x 2,048 x 768, 32 rows 9 / 14; 4,096 x 11,008 x 4,096, one row
+// 47 / 74, 32 rows 55 / 58; behind with 32 rows of 512 x 2,048 x 16,384 29 / 20, 4,096 x 14,336 x 4,096 82 / 70.
+bool few_rows(int64_t rows, int64_t in, int64_t mid, int64_t out) {
+  return rows <= 16 || (rows <= 32 && out <= 4096 && in * mid <= int64_t(48) << 20);
+}
 
 struct GatedFeedForwardBackward : public torch::autograd::Node {
   SavedVariable x, w_gate, w_up, w_down, hidden, gate, up, low;   // low: of bf16 (tgt_gated_hidden)
@@ -364,7 +366,7 @@ std::optional<at::Tensor> gated_feed_forward(const at::Tensor& x, const at::Tens
     sizes.back() = out;
     y = fresh(sizes, x);
     void* const stream = stream_of(x);
-    if (type == TGT_BF16 && !record && few_rows(rows, in, mid)) {
+    if (type == TGT_BF16 && !record && few_rows(rows, in, mid, out)) {
       check(tgt_gated_few_rows(ptr(xc), ptr(wgc), ptr(wuc), ptr(wdc), ptr(rc), rows, int(in), int(mid), int(out), act, ptr(h), ptr(y),
                                stream));
       return y;
