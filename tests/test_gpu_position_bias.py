@@ -54,6 +54,30 @@ def test_bias_and_gradient(edges, heads, buckets, distance, both_ways, ids):
         _check(table, list_.to(ids).cuda(), positions.to(kind).cuda(), distance, both_ways, dbias)
 
 
+@pytest.mark.parametrize("heads,buckets,ids,places", [(4, 128, torch.int64, torch.int64), (8, 64, torch.int64, torch.int32), (8, 4, torch.int32, torch.int64),
+                                                      (16, 33, torch.int32, torch.int32), (8, 130, torch.int64, torch.int64)])
+def test_many_edges(heads, buckets, ids, places):
+    """Lists long enough for the table in shared memory, odd ones, with and without positions, some ids outside them."""
+    from torchgt_b200.position_bias import bucket_borders, edge_position_bias
+    gen = torch.Generator().manual_seed(heads * buckets)
+    edges, nodes, both = 1310003 + heads, 5000, buckets % 2 == 0
+    list_ = torch.randint(0, nodes, (2, edges), generator=gen)
+    positions = torch.randint(-300, 300, (nodes,), generator=gen)
+    table = torch.randn(buckets, heads, generator=gen)
+    borders = bucket_borders(buckets, 200, both)
+    for where in (None, positions):
+        ends = list_ if where is None else where[list_]
+        want = table[_bucket(ends[0] - ends[1], borders, both)]
+        got = edge_position_bias(table.cuda(), list_.to(ids).cuda(), None if where is None else where.to(places).cuda(), 200, both)
+        assert torch.equal(got.cpu(), want)
+    wrong = list_.clone()
+    wrong[0, 7], wrong[1, edges - 1], wrong[1, edges // 2] = -1, nodes, nodes + 100
+    got = edge_position_bias(table.cuda(), wrong.to(ids).cuda(), positions.to(places).cuda(), 200, both).cpu()
+    bad = torch.zeros(edges, dtype=torch.bool)
+    bad[[7, edges - 1, edges // 2]] = True
+    assert torch.equal(got[~bad], want[~bad]) and bool(got[bad].isnan().all())
+
+
 def test_every_border_is_met_exactly():
     """Distances around every border, with one node at each place."""
     from torchgt_b200.position_bias import bucket_borders

@@ -11,8 +11,8 @@
 // group, head), so no two of them share a word or a bank, and what a hub's bucket costs is what any costs.  The sums
 // of a CTA's warps and then of the CTAs are added in a fixed order: no atomics, the same bits every time.  Both directions are bound by the
 // ids and the rows of bias; the forward keeps the buckets, 2 bytes an edge in the place of the 16 of two ids.
-// us, 18.2 M edges x 8 heads, 870,001 positions: forward 230 (910 MB; without positions 151: two random reads an edge keep the L1 76 %
-// busy), backward 130 and 9 for the last sums (620 MB); 526,450 edges 8.5, 8.4 and 4.5.
+// us, 18.2 M edges x 8 heads, 870,001 positions: forward 217 (910 MB; without positions 146: two random reads an edge keep the L1's
+// tags busy), backward 130 and 9 for the last sums (620 MB); 526,450 edges 8.5, 8.4 and 4.5.
 #include "tgt_common.cuh"
 
 namespace tgt {
@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kMostBuckets = 512, kMostHeads = 256;
 constexpr int kBiasThreads = 256;
+constexpr int bias_threads(bool shared) { return shared ? 1024 : kBiasThreads; }
 constexpr uint16_t kNoBucket = 0xffff;      // of an edge with an id outside the positions
 
 struct BiasFwd {
@@ -53,14 +54,23 @@ __device__ __forceinline__ int bucket_of(const BiasFwd& p, const int32_t* border
   return n + (s > d ? p.behind : 0);
 }
 
-template <typename Id, typename Pos, int VEC>
-__global__ void __launch_bounds__(kBiasThreads) position_bias_kernel(const __grid_constant__ BiasFwd p) {
+// SHARED: heads / 4 divides 8, and the table lies in shared memory, a row as the eight pieces of 16 bytes that the lanes of a
+// transaction take, each from banks of its own.
+template <typename Id, typename Pos, int VEC, bool SHARED>
+__global__ void __launch_bounds__(bias_threads(SHARED), 2048 / bias_threads(SHARED)) position_bias_kernel(const __grid_constant__ BiasFwd p) {
+  constexpr int kThreads = bias_threads(SHARED);
   __shared__ int32_t s_borders[kMostBuckets];
-  for (int i = threadIdx.x; i < p.n_borders; i += kBiasThreads) s_borders[i] = p.borders[i];
-  __syncthreads();
+  extern __shared__ __align__(16) float4 s_table[];          // SHARED: [buckets][8]
   const int lane = threadIdx.x % 32, pieces = p.heads / VEC;
-  const int64_t warps = int64_t(gridDim.x) * (kBiasThreads / 32);
-  for (int64_t e0 = (int64_t(blockIdx.x) * (kBiasThreads / 32) + threadIdx.x / 32) * 32; e0 < p.n_edges; e0 += warps * 32) {
+  for (int i = threadIdx.x; i < p.n_borders; i += kThreads) s_borders[i] = p.borders[i];
+  if constexpr (SHARED) {
+    const int buckets = (p.n_borders + 1) * (p.behind > 0 ? 2 : 1);
+    for (int i = threadIdx.x; i < buckets * 8; i += kThreads)
+      s_table[i] = __ldg(reinterpret_cast<const float4*>(p.table) + i / 8 * pieces + i % 8 % pieces);
+  }
+  __syncthreads();
+  const int64_t warps = int64_t(gridDim.x) * (kThreads / 32);
+  for (int64_t e0 = (int64_t(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32) * 32; e0 < p.n_edges; e0 += warps * 32) {
     const int64_t e = e0 + lane;
     int bucket = kNoBucket;
     if (e < p.n_edges) {
@@ -77,7 +87,8 @@ __global__ void __launch_bounds__(kBiasThreads) position_bias_kernel(const __gri
       const float nan = __int_as_float(0x7fffffff);
       if constexpr (VEC == 4) {
         float4 v = make_float4(nan, nan, nan, nan);
-        if (b != kNoBucket) v = __ldg(reinterpret_cast<const float4*>(p.table) + b * pieces + (piece - of * pieces));
+        if (b != kNoBucket)
+          v = SHARED ? s_table[b * 8 + lane % 8] : __ldg(reinterpret_cast<const float4*>(p.table) + b * pieces + (piece - of * pieces));
         __stcs(reinterpret_cast<float4*>(out) + piece, v);
       } else {
         out[piece] = b != kNoBucket ? __ldg(p.table + b * pieces + (piece - of * pieces)) : nan;
@@ -218,14 +229,21 @@ int check_sizes(int64_t n_edges, int n_buckets, int heads) {
   return TGT_OK;
 }
 
+// The table in the L1 / in shared memory, where many edges pay for large CTAs and for laying it out, us: 18.2 M edges, 8 heads 230 / 217;
+// 4 M, 64,000 positions, 4 heads 46.7 / 45.5, 8 51.9 / 48.6, 16 66 / 62, 32 98 / 105; 1.2 M, 8 heads 17.3 / 16.3; 526,450 9.5 / 9.9; 45,056
+// 3.4 / 4.2.  (The next edges' ids asked for a turn ahead: 217 -> 211 with positions, without 146 -> 156.)
+constexpr int kSharedBuckets = 128;
 template <typename Id, typename Pos>
 int launch_forward(const BiasFwd& p, cudaStream_t stream) {
-  const int64_t want = (p.n_edges + kBiasThreads - 1) / kBiasThreads, most = int64_t(sm_count()) * (2048 / kBiasThreads);
+  const bool wide = p.heads % 4 == 0 && aligned16(p.table) && aligned16(p.bias);
+  const int buckets = (p.n_borders + 1) * (p.behind > 0 ? 2 : 1);
+  const bool shared = wide && 16 % p.heads == 0 && buckets <= kSharedBuckets && p.n_edges >= int64_t(8192) * sm_count();
+  const int threads = bias_threads(shared);
+  const int64_t want = (p.n_edges + threads - 1) / threads, most = int64_t(sm_count()) * (2048 / threads);
   const unsigned grid = unsigned(want < most ? want : most);
-  if (p.heads % 4 == 0 && aligned16(p.table) && aligned16(p.bias))
-    position_bias_kernel<Id, Pos, 4><<<grid, kBiasThreads, 0, stream>>>(p);
-  else
-    position_bias_kernel<Id, Pos, 1><<<grid, kBiasThreads, 0, stream>>>(p);
+  if (shared) position_bias_kernel<Id, Pos, 4, true><<<grid, threads, buckets * 128, stream>>>(p);
+  else if (wide) position_bias_kernel<Id, Pos, 4, false><<<grid, threads, 0, stream>>>(p);
+  else position_bias_kernel<Id, Pos, 1, false><<<grid, threads, 0, stream>>>(p);
   TGT_CHECK_CUDA(cudaGetLastError());
   return TGT_OK;
 }
