@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       const int n0 = FINISH == kGated ? n_tile * (BN / 2) : n_tile * BN + rank * kRowsB;
       for (int chunk = work.k0; chunk < work.k1; ++chunk) {
         if (!(ok = tma::wait(s_empty + stage, phase))) break;
-        if (tma::elect()) {
+        if (tc::elect()) {
           if (rank == 0) tma::arrive_expecting(s_full + stage, kCtas * kStage);
           const uint32_t bar = full + stage * 8;
           const bool second = chunk >= p.source_chunks;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           if (!(ok = tma::wait(s_full + stage, phase))) break;
           tc::fence_after_barrier();
           const uint32_t a = s_ring + stage * kStage, b = a + kBytesA;
-          if (tma::elect()) {
+          if (tc::elect()) {
 #pragma unroll
             for (int k = 0; k < kChunk / 16; ++k) {
               const uint64_t da = A_MN ? tc::mn_major(a + 2048 * k, 8192) : tc::k_major(a + 32 * k);
@@ -344,14 +344,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
         if (!ok) break;
-        if (tma::elect()) commit<PAIR>(s_sums + half);
+        if (tc::elect()) commit<PAIR>(s_sums + half);
         __syncwarp();
         if (half == 1) taken ^= 1;
         half ^= 1;
       }
       if (!ok) {
         if (lane == 0) tc::report_expired_wait(p.expired);
-        if (tma::elect()) commit<PAIR>(s_drained);       // products that still run write to the memory given back
+        if (tc::elect()) commit<PAIR>(s_drained);       // products that still run write to the memory given back
         __syncwarp();
         tc::wait(s_drained, 0);
       }

@@ -20,7 +20,7 @@
 // Relative error against 64 bits, normal operands: 64 long 7e-8 (FMA 1.1e-7, library 1.5e-7), 128 long 1.2e-7 (1.5e-7, 2.0e-7),
 // 1024 long 1.2e-7 (4.1e-7, 5.7e-7; with one running sum 1.0e-6), three gradients 64 long 7.6e-8 (library 1.5e-7, one running
 // sum 1.7e-7); operands of one sign, 128 long 1.8e-7 (9e-8, 1.7e-7), 1024 long 1.6e-7 (2.5e-7, 4.9e-7; 2.2e-6).  Six chunks at
-// most are one launch because their weights fit shared memory; 1024 x 1024 over 8,192 rows in three launches 282 us.
+// most are one launch because their weights fit shared memory; 1024 x 1024 over 8,192 rows in three launches 247 us (282 with the products issued by a lane alone).
 #include "linear_rows.cuh"
 #include "tensor_core.cuh"
 
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, LONG ? 1 : 2) split_gemm_kernel(cons
     for (; tile < tiles; tile += walkers) {
       for (int chunk = 0; chunk < p.chunks; ++chunk) {
         if (!__syncthreads_and(true)) goto finished;        // the workers' pieces are in place
-        if (lane == 0) {
+        if (tc::elect()) {
           tc::fence_after_barrier();
           const uint32_t w = s_w + chunk * (3 * kPieceW);
 #pragma unroll

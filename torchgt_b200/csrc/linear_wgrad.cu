@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kWgThreads, 2) linear_wgrad_kernel(const __gri
     tc::fence_before_barrier();
     ok = __syncthreads_and(ok);
     if (!ok) break;
-    if (tid == 64) {                                 // of a warp that does not drain
+    if (warp == 2 && tc::elect()) {                  // of a warp that does not drain
       tc::fence_after_barrier();
       constexpr uint32_t one = tc::instruction(128, 64, true, true);
 #pragma unroll

@@ -61,6 +61,13 @@ constexpr uint32_t instruction(int m, int n, bool a_mn_major, bool b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(a_mn_major) << 15) | (uint32_t(b_mn_major) << 16) |
          (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
+// One lane of a warp that is together, the same every time; the compiler knows that it is one, and keeps what
+// an instruction takes in uniform registers.
+__device__ __forceinline__ bool elect() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 // D[m][n] (+)= sum over 16 k; one thread issues it
 __device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
   asm volatile(

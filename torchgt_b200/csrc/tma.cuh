@@ -29,12 +29,6 @@ __device__ __forceinline__ void barrier_init(uint64_t* bar, int arrivals) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tc::smem_address(bar)), "r"(arrivals) : "memory");
 }
 __device__ __forceinline__ void barriers_ready() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
-// One lane of a warp that is together, the same every time; the compiler knows that it is one.
-__device__ __forceinline__ bool elect() {
-  uint32_t one;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
-  return one != 0;
-}
 // tc::wait by a whole warp, without the clock where the phase is complete or about to be: what feeds the tensor cores waits for
 // every 64 of k.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t phase) {
