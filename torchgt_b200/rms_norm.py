@@ -15,8 +15,8 @@ from .linear import plain_call, unobserved
 
 
 def _eps(x: torch.Tensor, eps: Optional[float]) -> float:
-    """``torch.nn.RMSNorm``'s default (of whole numbers any: torch refuses them)."""
-    return eps if eps is not None else torch.finfo(x.dtype).eps if x.is_floating_point() else 0.0
+    """``torch.nn.RMSNorm``'s default: the machine epsilon of the type that rows of ``x``'s are computed in."""
+    return eps if eps is not None else torch.finfo(torch.float64 if x.dtype == torch.float64 else torch.float32).eps
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None) -> torch.Tensor:
