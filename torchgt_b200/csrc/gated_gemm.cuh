@@ -116,7 +116,7 @@ __device__ __forceinline__ uint32_t first_ctas(uint32_t address) {
   if constexpr (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(address) : "r"(address));
   return address;
 }
-__device__ __forceinline__ void cluster_barrier() {              // every thread of all CTAs
+__device__ __forceinline__ void cluster_barrier() {              // every thread of all CTAs, a warp together
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // 16 bytes of shared memory of CTA `cta` of the cluster, at the place that `address` is in this one's
@@ -401,6 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     };
     auto sums = [&](uint32_t at, float (&v)[32]) {
       uint32_t r[2][16];
+      __syncwarp();                                      // lanes without a row or a column have left the stores before this
       tc::read16(at, r[0]);
       tc::read16(at + 16, r[1]);
       tc::reads_done();
@@ -621,6 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       }
       store(p.out[0], [&](int i) { return f32_to_bf16x2(v[i], v[i + 1]); });
     }
+    __syncwarp();                                        // of lanes that left the loop apart: a barrier takes whole warps
     cluster_barrier();                                   // nobody reads another's sums any more
   }
   if constexpr (PAIR) cluster_barrier();                 // neither uses the other's shared or tensor memory any more

@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(kThreads, LONG ? 1 : 2) split_gemm_kernel(cons
   auto finish = [&](int64_t of, uint32_t sums) {
     const int64_t row0 = of * kRows + warp % 4 * 32;
     sums += (uint32_t(warp % 4 * 32) << 16) + warp / 4 * 32;
+    __syncwarp();                                           // lanes come from waits of their own
 #pragma unroll 1
     for (int j = 0; j < 32; j += kBlockCols) {
       uint32_t big[16], small[16];
@@ -373,6 +374,7 @@ finished:
   __syncthreads();
   if (warp == 0) {
     if (failed >= 0) tc::wait(s_done, phase ^ 1);           // products that still run write to the memory given back
+    __syncwarp();
     tc::release<2 * kHalf>(tmem);
   }
 }

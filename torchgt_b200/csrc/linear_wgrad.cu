@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(kWgThreads, 2) linear_wgrad_kernel(const __gri
   auto drain = [&](int n) {                        // large products of this CTA's n-th chunk, counted from 0
     ok = tc::wait(s_done + n % 2, n / 2 % 2) && ok;
     tc::fence_after_barrier();
+    __syncwarp();                                  // lanes come from waits of their own
     if (warp % 4 < 2) {
 #pragma unroll
       for (int j = 0; j < 32; j += 16) {

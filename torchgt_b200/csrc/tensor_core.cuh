@@ -28,7 +28,8 @@ __device__ __forceinline__ void release(uint32_t address) {   // by the warp tha
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "n"(COLS));
 }
 
-// 16 consecutive fp32 columns of the calling warp's 32 lanes (warp w of a CTA reaches lanes 32 (w % 4) and up)
+// 16 consecutive fp32 columns of the calling warp's 32 lanes (warp w of a CTA reaches lanes 32 (w % 4) and up).  Like the allocation
+// and the waits for it, for a warp that is together: __syncwarp() stands between it and code that lanes leave apart.
 __device__ __forceinline__ void read16(uint32_t address, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
