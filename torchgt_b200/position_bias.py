@@ -46,17 +46,22 @@ def bucket_borders(num_buckets: int, max_distance: int, bidirectional: bool) -> 
 
 
 def _as_operations(table, edge_index, positions, borders, bidirectional):
-    """The same from operations that tracers, compilers and ``torch.func`` can record; an id outside the positions is torch's
-    error."""
+    """The same from operations that tracers, compilers and ``torch.func`` can record."""
     source, destination = edge_index.long().unbind(0)
+    outside = None
     if positions is not None:
-        source, destination = positions.long()[source], positions.long()[destination]
+        nodes = positions.shape[0]
+        outside = (source < 0) | (source >= nodes) | (destination < 0) | (destination >= nodes)
+        positions = positions.long() if nodes > 0 else positions.new_zeros(1).long()
+        last = positions.shape[0] - 1            # no index reaches past it: on a GPU torch's error ends the process's context
+        source, destination = positions[source.clamp(0, last)], positions[destination.clamp(0, last)]
     offset = source - destination
     distance = offset.abs() if bidirectional else (-offset).clamp(min=0)
     bucket = torch.bucketize(distance, torch.tensor(borders, device=table.device), right=True)
     if bidirectional:
         bucket = bucket + (offset > 0).long() * (len(borders) + 1)
-    return torch.nn.functional.embedding(bucket, table)
+    bias = torch.nn.functional.embedding(bucket, table)
+    return bias if outside is None else torch.where(outside.unsqueeze(-1), float("nan"), bias)
 
 
 def edge_position_bias(table: torch.Tensor, edge_index: torch.Tensor, positions: Optional[torch.Tensor] = None,
