@@ -65,3 +65,31 @@ def test_ids_outside_the_positions_under_vmap():
     moved = torch.func.vmap(lambda p: edge_position_bias(table, edges, p))(torch.stack([positions, positions.flip(0)]))
     assert _same(moved[0], want) and _same(moved[1], edge_position_bias(table, edges, positions.flip(0)))
     torch.cuda.synchronize()
+
+
+def _far_places():
+    places = [0, 1, -1, 2 ** 40, -2 ** 40, 2 ** 62, -2 ** 62, -2 ** 62 - 1, 2 ** 63 - 1, -2 ** 63, -2 ** 63 + 1]
+    n = len(places)
+    return torch.cartesian_prod(torch.arange(n), torch.arange(n)).t().contiguous(), torch.tensor(places), torch.arange(32.)[:, None].repeat(1, 2)
+
+
+@pytest.mark.parametrize("both_ways", [True, False])
+def test_positions_at_the_ends_of_64_bits(both_ways):
+    """Differences that 64 bits do not hold, and the one whose negative they do not."""
+    edges, positions, table = _far_places()
+    want = _defined(table, edges, positions, both_ways=both_ways)
+    assert torch.equal(_recorded(table, edges, positions, both_ways=both_ways), want)
+    assert torch.equal(_recorded(table, positions[edges], None, both_ways=both_ways), want)   # without positions an id is its place
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("both_ways", [True, False])
+def test_positions_at_the_ends_of_64_bits_in_the_kernels(both_ways):
+    from torchgt_b200 import edge_position_bias
+    edges, positions, table = _far_places()
+    want = _defined(table, edges, positions, both_ways=both_ways)
+    for ids, where in ((edges, positions.cuda()), (positions[edges], None)):
+        got = edge_position_bias(table.cuda(), ids.cuda(), where, bidirectional=both_ways)
+        assert torch.equal(got.cpu(), want)
+        wrapped = torch.func.vmap(lambda t: edge_position_bias(t, ids.cuda(), where, bidirectional=both_ways))(table.cuda()[None])   # noqa: B023
+        assert torch.equal(wrapped[0].cpu(), want)

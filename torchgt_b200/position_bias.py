@@ -55,11 +55,14 @@ def _as_operations(table, edge_index, positions, borders, bidirectional):
         positions = positions.long() if nodes > 0 else positions.new_zeros(1).long()
         last = positions.shape[0] - 1            # no index reaches past it: on a GPU torch's error ends the process's context
         source, destination = positions[source.clamp(0, last)], positions[destination.clamp(0, last)]
-    offset = source - destination
-    distance = offset.abs() if bidirectional else (-offset).clamp(min=0)
+    behind = source > destination
+    distance = torch.maximum(source, destination) - torch.minimum(source, destination)
+    distance = torch.where(distance < 0, torch.iinfo(torch.int64).max, distance)         # 2^63 and more
+    if not bidirectional:
+        distance = distance.masked_fill(behind, 0)
     bucket = torch.bucketize(distance, torch.tensor(borders, device=table.device), right=True)
     if bidirectional:
-        bucket = bucket + (offset > 0).long() * (len(borders) + 1)
+        bucket = bucket + behind.long() * (len(borders) + 1)
     bias = torch.nn.functional.embedding(bucket, table)
     return bias if outside is None else torch.where(outside.unsqueeze(-1), float("nan"), bias)
 
