@@ -47,10 +47,14 @@ def wgrad(dy: torch.Tensor, x: torch.Tensor, with_bias: bool = True):
     return dw, db
 
 
+def untraced(*tensors) -> bool:
+    """No tracer, compiler or tensor subclass wants to see PyTorch's own operation."""
+    return not (torch.compiler.is_compiling() or torch.jit.is_tracing() or has_torch_function_variadic(*tensors))
+
+
 def plain_call(*tensors) -> bool:
-    """No tracer, compiler, autocast or tensor subclass wants to see PyTorch's own operation."""
-    return not (torch.compiler.is_compiling() or torch.jit.is_tracing() or torch.is_autocast_enabled("cuda") or
-                has_torch_function_variadic(*tensors))
+    """:func:`untraced`, and no autocast either."""
+    return not torch.is_autocast_enabled("cuda") and untraced(*tensors)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias) -> torch.Tensor:

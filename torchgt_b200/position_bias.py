@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _cabi
-from .linear import plain_call
+from .linear import untraced
 
 _MOST_BUCKETS, _MOST_HEADS = 512, 256
 _IDS = (torch.int64, torch.int32)
@@ -91,7 +91,7 @@ def edge_position_bias(table: torch.Tensor, edge_index: torch.Tensor, positions:
     if positions is not None and positions.dim() != 1:
         raise ValueError("positions must be [N]")
     borders = bucket_borders(table.shape[0], max_distance, bool(bidirectional))
-    if plain_call(*tensors):
+    if untraced(*tensors):               # under autocast too: nothing here is of a type that it changes
         bias = _cabi.native().edge_position_bias(table, edge_index, positions, borders, bool(bidirectional))
         if bias is not None:
             return bias
