@@ -12,6 +12,7 @@ about a distance."""
 from __future__ import annotations
 
 import functools
+import operator
 from typing import Optional
 
 import torch
@@ -23,9 +24,13 @@ _MOST_BUCKETS, _MOST_HEADS = 512, 256
 _IDS = (torch.int64, torch.int32)
 
 
-@functools.lru_cache(maxsize=64)
 def bucket_borders(num_buckets: int, max_distance: int, bidirectional: bool) -> tuple:
     """The smallest distance of every bucket of one direction but the first."""
+    return _borders(operator.index(num_buckets), operator.index(max_distance), bool(bidirectional))
+
+
+@functools.lru_cache(maxsize=64)
+def _borders(num_buckets, max_distance, bidirectional):
     count = num_buckets // 2 if bidirectional else num_buckets
     if num_buckets > _MOST_BUCKETS or count < 2 or (bidirectional and num_buckets % 2):
         raise ValueError(f"num_buckets must be {'even and 4' if bidirectional else '2'} to {_MOST_BUCKETS}; got {num_buckets}")
@@ -90,7 +95,7 @@ def edge_position_bias(table: torch.Tensor, edge_index: torch.Tensor, positions:
         raise ValueError("edge_index must be [2, E]")
     if positions is not None and positions.dim() != 1:
         raise ValueError("positions must be [N]")
-    borders = bucket_borders(table.shape[0], max_distance, bool(bidirectional))
+    borders = bucket_borders(table.shape[0], max_distance, bidirectional)
     if untraced(*tensors):               # under autocast too: nothing here is of a type that it changes
         bias = _cabi.native().edge_position_bias(table, edge_index, positions, borders, bool(bidirectional))
         if bias is not None:
@@ -104,7 +109,7 @@ class RelativePositionBias(torch.nn.Module):
 
     def __init__(self, num_heads: int, num_buckets: int = 32, max_distance: int = 128, bidirectional: bool = True):
         super().__init__()
-        bucket_borders(num_buckets, max_distance, bool(bidirectional))      # refuses what it cannot make
+        bucket_borders(num_buckets, max_distance, bidirectional)            # refuses what it cannot make
         self.num_heads, self.num_buckets = num_heads, num_buckets
         self.max_distance, self.bidirectional = max_distance, bool(bidirectional)
         self.weight = torch.nn.Parameter(torch.empty(num_buckets, num_heads))
