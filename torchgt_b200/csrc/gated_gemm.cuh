@@ -191,7 +191,8 @@ __device__ __forceinline__ float sigmoid(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
   return s;
 }
-// act(x), and with SLOPE its derivative.  The results are rounded to 8 bits: the fast exponential and quotient are 2^-20 off.
+// act(x), and with SLOPE its derivative.  The results are rounded to 8 bits: the fast exponential and quotient are 2^-20 off, and by
+// the rounding of the power |x| 2^-23 more (2^-17 at -64).
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ float activate(float x, float& slope) {
   if constexpr (ACT == TGT_ACT_SILU) {

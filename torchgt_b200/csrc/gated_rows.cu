@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(32 * WARPS) few_rows_kernel(const FewRows p) {
     const int row = n * 8 + 2 * (l % 4) + i % 2, col = col0 + m * kSetCols + l / 4 + (i / 2) * 8;
     if (row >= p.rows || col >= p.cols) continue;
     if (GATED) {
+      // 2^-20 + |s| 2^-23 off (the power's rounding), next to a rounding to 8 bits
       const float a = p.act == TGT_ACT_SILU ? s / (1.f + __expf(-s)) : p.act == TGT_ACT_GELU ? gelu(s) : relu(s);
       s = a * u;
     } else if (p.add != nullptr) {

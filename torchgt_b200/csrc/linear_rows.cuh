@@ -17,9 +17,10 @@ __device__ __forceinline__ float gelu_slope(float x) {
   return normal_cdf(x) + x * (0.39894228040143267794f * expf(-0.5f * x * x));
 }
 
-// 1 / (1 + exp(-x)) to about 2^-22, from the mathematics: exp(-y) = 2^t exp(r) with t = -y log2(e) as it rounds and r = -y - t ln(2)
-// what that leaves, at most 1e-5, so exp(r) is 1 + r; then the approximate reciprocal (1 unit).  0 below -87, where the quotient
-// leaves the normal numbers, and for whatever a NaN makes of it.
+// 1 / (1 + exp(-x)) to 2^-20, from the mathematics: exp(-y) = 2^t exp(r) with t = -y log2(e) as it rounds and r = -y - t ln(2)
+// what that leaves, at most 1e-5, so exp(r) is 1 + r; then the approximate reciprocal (1 unit).  0 below -87, next to where the
+// quotient leaves the normal numbers (2^-125 is lost), and for whatever a NaN makes of it.  x logistic(x) at 400,001 places from -110 to
+// 110: 2^-21.3 from 64 bits at most.
 __device__ __forceinline__ float logistic(float x) {
   const float y = fminf(fmaxf(x, -87.f), 87.f);
   const float t = -y * 1.44269504088896341f, r = fmaf(-t, 0.693147180559945309f, -y);
