@@ -569,8 +569,9 @@ TGT_API int tgt_embedding_sum_grad(const float* dout, const int64_t* ids, int64_
  * NULL) receives v, rest (int8, may be NULL; of a bf16 sum) what its rounding took, rstd (may be NULL) one fp32 value a row.  hidden is 1 to 16384 (TGT_ERR_UNSUPPORTED above).  Rows of
  * whole 16-byte pieces from 16-byte boundaries on move in such pieces, others value by value.  What is written must not overlap
  * what is read.
- *   e4m3:     the same with y in 8 bits: scales [rows] = max(max |y| / 448, 2^-126) and values [rows, hidden] = y / scale, to
- *             the nearest e4m3 number.  A row with a NaN or an infinity has a NaN scale.
+ *   e4m3:     the same with y in 8 bits: scales [rows] = max(max |y| / 448, 2^-126) and values [rows, hidden] = y times the
+ *             rounded 1 / scale, to the nearest e4m3 number (where y / scale lies next to the middle of two, either).  A row with
+ *             a NaN or an infinity has a NaN scale.
  *   backward: dx = rstd (dy weight - u mean(dy weight u)) + dsum with u = v rstd, dsum (may be NULL) the gradient of sum, v
  *             what the forward had as x or stored as sum (with rest, or NULL); dweight [hidden] = sum over rows of dy u, fixed order.
  */
@@ -604,8 +605,10 @@ TGT_API int tgt_edge_position_bias_grad(const float* dbias, const uint16_t* buck
  * Gated feed-forward block, h = act(x w_gate^T) * (x w_up^T), y = h w_down^T + add, and its gradients, with act TGT_ACT_SILU,
  * TGT_ACT_GELU (exact) or TGT_ACT_RELU; w_gate and w_up are [mid, in], w_down is [out, mid], all tensors packed and of `dtype`,
  * 16-byte aligned.  TGT_BF16: products on the tensor cores with fp32 sums, the activation and the product of the two
- * projections in fp32 before h is rounded; widths multiples of 8, at most 65536.  TGT_F32: the products of tgt_linear_rows
- * and what follows in a kernel of its own; in and mid multiples of 64, out of 4, at most 1024 (TGT_ERR_UNSUPPORTED otherwise).
+ * projections in fp32 before h is rounded; widths multiples of 8, at most 65536.  TGT_F32: the split products of tgt_linear_rows,
+ * with the gate and its gradient in their finish, or for few rows and long reductions in kernels of their own; widths multiples of
+ * 4, at most 1024, in_features of weight_grad a multiple of 64: in and mid are of 64 where gradients of the weights are wanted
+ * (TGT_ERR_UNSUPPORTED otherwise).
  *   hidden:      h, and where gate is not NULL (TGT_F32: never) gate = x w_gate^T and up = x w_up^T as the gradients need them:
  *                in bf16 the upper 16 bits of their fp32 sums, and in low [rows, mid] the next 8 bits of both (gate's in the
  *                lower byte); in fp32 the sums, and low is not used

@@ -54,8 +54,8 @@ __device__ __forceinline__ int bucket_of(const BiasFwd& p, const int32_t* border
   return n + (s > d ? p.behind : 0);
 }
 
-// SHARED: heads / 4 divides 8, and the table lies in shared memory, a row as the eight pieces of 16 bytes that the lanes of a
-// transaction take, each from banks of its own.
+// SHARED: 4, 8 or 16 heads, and the table lies in shared memory, a row as the eight pieces of 16 bytes that the lanes of a
+// transaction take, each from banks of its own: its one, two or four pieces again and again.
 template <typename Id, typename Pos, int VEC, bool SHARED>
 __global__ void __launch_bounds__(bias_threads(SHARED), 2048 / bias_threads(SHARED)) position_bias_kernel(const __grid_constant__ BiasFwd p) {
   constexpr int kThreads = bias_threads(SHARED);

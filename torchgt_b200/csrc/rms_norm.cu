@@ -2,7 +2,7 @@
 //
 //   v = x + residual,  rstd = 1 / sqrt(mean(v^2) + eps),  y = v rstd w,  sum = v
 //   g = dy w,  u = v rstd:   dx = rstd (g - u mean(g u)) + dsum,  dw = sum over rows of dy u
-//   8 bits:  scale = max(max |y| / 448, 2^-126),  values = e4m3(y / scale)
+//   8 bits:  scale = max(max |y| / 448, 2^-126),  values = e4m3(y (1 / scale)), 1 / scale rounded: a division less per value
 //
 // All of it in fp32, rounded once where it is stored; y comes from v before v is rounded for the residual stream.  In bf16 the
 // forward can leave the next 8 bits of v beside the rounded sum for the backward: with the sum alone its rounding is in dw next
