@@ -42,8 +42,14 @@ struct RmsNormRowsBackward : public torch::autograd::Node {
   double eps = 0;
 
   // With create_graph the gradient is itself differentiated, with is_grads_batched there are many: the formula as operations.
-  variable_list recorded(const at::Tensor& dy_, const at::Tensor& ds, const at::Tensor& v_, const at::Tensor& w_) {
-    const at::Tensor v = v_.to(at::kFloat), w = w_.to(at::kFloat);
+  variable_list recorded(const at::Tensor& dy_, const at::Tensor& ds, const at::Tensor& v_, const at::Tensor& w_,
+                         const at::Tensor& rest_) {
+    const at::Tensor w = w_.to(at::kFloat);
+    at::Tensor v = v_.to(at::kFloat);
+    if (rest_.defined()) {   // the sum before it was rounded, as the kernel takes it, with the rounded sum's derivative
+      const at::Tensor rounded = v.detach(), whole = (rounded.view(at::kInt) + rest_.to(at::kInt) * 256).view(at::kFloat);
+      v = whole + at::where(rounded.isfinite(), v - rounded, at::zeros_like(rounded));
+    }
     const at::Tensor r = (v * v).mean(-1, true).add(eps).rsqrt(), u = v * r;
     at::Tensor dx, dw;
     if (dy_.defined()) {
@@ -65,7 +71,7 @@ struct RmsNormRowsBackward : public torch::autograd::Node {
     const at::Tensor v = with_residual ? normalised.unpack(shared_from_this()) : normalised.unpack();
     const at::Tensor w = weight.unpack(), rstd_ = rstd.unpack(), rest_ = rest.unpack();
     if (at::GradMode::is_enabled() || at::isTensorSubclassLike(grads[0]) || (ds.defined() && at::isTensorSubclassLike(ds)))
-      return recorded(grads[0], ds, v, w);
+      return recorded(grads[0], ds, v, w, rest_);
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(v.device());
     const at::Tensor dy = grads[0].contiguous(), vc = v.contiguous(), wc = w.contiguous();
