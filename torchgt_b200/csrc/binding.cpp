@@ -348,7 +348,7 @@ struct SparseGraphAttentionBackward : public torch::autograd::Node {
     const at::Tensor out_ = want_dbias && reads_out() ? out.unpack(shared_from_this()) : at::Tensor();
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(q_.device());
-    const at::Tensor dout = grads[0].contiguous();
+    const at::Tensor dout = packed(grads[0]);
     at::Tensor dq = at::empty_like(q_), dk = at::empty_like(k_), dv = at::empty_like(v_), dbias;
     if (want_dbias) dbias = at::empty_like(bias_);
     attention_backward(*graph, dout, q_, k_, v_, bias_, out_, z_, dq, dk, dv, dbias, heads, head_dim, dtype);
@@ -363,14 +363,14 @@ struct SparseGraphAttentionBackward : public torch::autograd::Node {
 
 }  // namespace
 
-at::Tensor attention_over_rows(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& bias,
+at::Tensor attention_over_rows(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& bias_in,
                                const std::shared_ptr<Graph>& graph, int heads, int head_dim) {
   // the node has no forward-mode formula: refuse a dual tensor rather than drop its tangent
-  for (const at::Tensor* t : {&q_in, &k_in, &v_in, &bias})
+  for (const at::Tensor* t : {&q_in, &k_in, &v_in, &bias_in})
     TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(*t),
                                 "sparse_graph_attention does not support forward-mode AD");
-  check_rows(*graph, q_in, k_in, v_in, bias, heads, head_dim);
-  const at::Tensor q = q_in.contiguous(), k = k_in.contiguous(), v = v_in.contiguous();
+  check_rows(*graph, q_in, k_in, v_in, bias_in, heads, head_dim);
+  const at::Tensor q = packed(q_in), k = packed(k_in), v = packed(v_in), bias = bias_in.defined() ? bias_in.resolve_neg() : bias_in;
   const int dtype = dtype_of(q);
   const c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out, z;
@@ -439,7 +439,7 @@ std::vector<std::optional<at::Tensor>> backward_pass(const at::Tensor& dout, con
   const at::Tensor bias_ = bias.value_or(at::Tensor());
   at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v), dbias;
   if (want_dbias) dbias = at::empty_like(bias_);
-  attention_backward(*graph, dout.contiguous(), q, k, v, bias_, out.value_or(at::Tensor()), z, dq, dk, dv, dbias, int(q.size(1)),
+  attention_backward(*graph, packed(dout), q, k, v, bias_, out.value_or(at::Tensor()), z, dq, dk, dv, dbias, int(q.size(1)),
                      int(q.size(2)), dtype_of(q));
   return {dq, dk, dv, want_dbias ? std::optional<at::Tensor>(dbias) : std::nullopt};
 }

@@ -55,6 +55,9 @@ using Unlocked = pybind11::call_guard<pybind11::gil_scoped_release>;
 
 void* stream_of(const at::Tensor& t);   // the current stream of t's device
 
+// What a kernel reads of t: its values side by side.  A lazily negated view (the imaginary part of a conjugate is one) counts as
+// contiguous while its memory has the other sign.
+inline at::Tensor packed(const at::Tensor& t) { return t.resolve_neg().contiguous(); }
 inline void* ptr(const at::Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
 inline float* fptr(const at::Tensor& t) { return static_cast<float*>(ptr(t)); }
 

@@ -74,8 +74,8 @@ struct RmsNormRowsBackward : public torch::autograd::Node {
       return recorded(grads[0], ds, v, w, rest_);
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(v.device());
-    const at::Tensor dy = grads[0].contiguous(), vc = v.contiguous(), wc = w.contiguous();
-    const at::Tensor dsum = ds.defined() ? ds.contiguous() : ds;
+    const at::Tensor dy = packed(grads[0]), vc = v.contiguous(), wc = w.contiguous();
+    const at::Tensor dsum = ds.defined() ? packed(ds) : ds;
     const int64_t hidden = w.numel(), rows = v.numel() / hidden;
     const at::Tensor dx = fresh(v.sizes(), dy), dw = fresh(w.sizes(), dy);
     size_t bytes = 0;
@@ -181,7 +181,7 @@ struct EdgePositionBiasBackward : public torch::autograd::Node {
     }
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(of.device());
-    const at::Tensor d = grads[0].contiguous(), dtable = fresh({n_buckets, heads}, d);
+    const at::Tensor d = packed(grads[0]), dtable = fresh({n_buckets, heads}, d);
     size_t bytes = 0;
     check(tgt_edge_position_bias_grad_scratch_bytes(edges, int(n_buckets), int(heads), &bytes));
     const at::Tensor scratch = scratch_of(bytes, d);
@@ -239,7 +239,7 @@ int activation_code(const std::string& name) {
 
 // contiguous, and copied when it is a view that starts off a 16-byte boundary (the kernels move 16 bytes at a time)
 at::Tensor kernel_ready(const at::Tensor& t) {
-  const at::Tensor c = t.contiguous();
+  const at::Tensor c = packed(t);
   return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0 ? c : c.clone();
 }
 

@@ -20,7 +20,7 @@ bool aligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_p
 
 // contiguous, and copied when it is a view that starts off a 16-byte boundary (the kernels move 16 bytes at a time)
 at::Tensor kernel_ready(const at::Tensor& t) {
-  at::Tensor c = t.contiguous();
+  at::Tensor c = packed(t);
   return aligned(c) ? c : c.clone();
 }
 
