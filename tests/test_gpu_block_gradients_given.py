@@ -1,7 +1,9 @@
 """The gradients that the operators of a block are given, in forms that autograd has for them: lazily negated ones, as the imaginary
-part of a conjugate is."""
+part of a conjugate is, and ones with tangents."""
 import pytest
 import torch
+
+from helpers import TOL_F32, rel_err
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +62,19 @@ def test_lazily_negated_inputs_of_the_attention(dtype):
         if name.startswith("attention"):
             values = [t.detach() for t in leaves]
             assert torch.equal(f(*[torch._neg_view(t) for t in values]), f(*[-t for t in values])), name
+
+
+def test_with_tangents():
+    """Forward-mode derivatives of a backward pass: it is linear in what it is given, so its tangent is the backward of the tangent."""
+    import torch.autograd.forward_ad as forward_ad
+    for name, f, leaves in _operators(torch.float32):
+        if not name.startswith(("norm", "sum", "gated", "bias")):
+            continue
+        y = f(*leaves)
+        dy, tangent = torch.randn_like(y), torch.randn_like(y)
+        want = [torch.autograd.grad(f(*leaves), leaves, t) for t in (dy, tangent)]
+        with forward_ad.dual_level():
+            for got, primal, slope in zip(torch.autograd.grad(f(*leaves), leaves, forward_ad.make_dual(dy, tangent)), *want):
+                parts = forward_ad.unpack_dual(got)
+                assert parts.tangent is not None, name
+                assert rel_err(parts.primal, primal) <= TOL_F32 and rel_err(parts.tangent, slope) <= TOL_F32, name

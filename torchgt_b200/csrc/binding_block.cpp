@@ -25,6 +25,12 @@ bool plain(const at::Tensor& t, const at::Device& device, at::ScalarType type) {
 bool kernel_type(at::ScalarType type) { return type == at::kFloat || type == at::kBFloat16; }
 int type_code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? TGT_F32 : TGT_BF16; }
 
+// A backward pass is the formula as operations, not kernels: it is itself differentiated (create_graph), there are many gradients at once
+// (is_grads_batched), or they carry tangents, which would be lost.
+bool as_operations(const at::Tensor& grad) {
+  return at::GradMode::is_enabled() || (grad.defined() && (at::isTensorSubclassLike(grad) || torch::autograd::isFwGradDefined(grad)));
+}
+
 // An uninitialised tensor next to `like`, straight from the allocator's function: the small calls are bound by the host, and on its
 // way through the dispatcher at::empty takes twice the time.
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
@@ -41,7 +47,6 @@ struct RmsNormRowsBackward : public torch::autograd::Node {
   bool with_residual = false;
   double eps = 0;
 
-  // With create_graph the gradient is itself differentiated, with is_grads_batched there are many: the formula as operations.
   variable_list recorded(const at::Tensor& dy_, const at::Tensor& ds, const at::Tensor& v_, const at::Tensor& w_,
                          const at::Tensor& rest_) {
     const at::Tensor w = w_.to(at::kFloat);
@@ -70,7 +75,7 @@ struct RmsNormRowsBackward : public torch::autograd::Node {
     if (!grads[0].defined()) return {ds, ds, at::Tensor()};              // only x + residual was used, or nothing
     const at::Tensor v = with_residual ? normalised.unpack(shared_from_this()) : normalised.unpack();
     const at::Tensor w = weight.unpack(), rstd_ = rstd.unpack(), rest_ = rest.unpack();
-    if (at::GradMode::is_enabled() || at::isTensorSubclassLike(grads[0]) || (ds.defined() && at::isTensorSubclassLike(ds)))
+    if (as_operations(grads[0]) || as_operations(ds))
       return recorded(grads[0], ds, v, w, rest_);
     const at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(v.device());
@@ -174,8 +179,7 @@ struct EdgePositionBiasBackward : public torch::autograd::Node {
     if (!grads[0].defined()) return variable_list(1);
     const at::Tensor of = buckets.unpack();
     const int64_t edges = of.numel(), heads = grads[0].size(-1);
-    // a second-order gradient is wanted, or many gradients at once (is_grads_batched)
-    if (at::GradMode::is_enabled() || at::isTensorSubclassLike(grads[0])) {
+    if (as_operations(grads[0])) {
       const at::Tensor known = of.ge(0).unsqueeze(-1), d = at::where(known, grads[0], at::zeros_like(grads[0]));
       return {at::zeros({n_buckets, heads}, grads[0].options()).index_add(0, of.clamp_min(0).to(at::kLong), d)};
     }
@@ -258,7 +262,6 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     return reporting([&] { return backward(grads); });
   }
-  // With create_graph the gradient is itself differentiated, with is_grads_batched there are many: the formula as operations.
   variable_list recorded(const at::Tensor& dy, const at::Tensor& x_, const at::Tensor& wg, const at::Tensor& wu,
                          const at::Tensor& wd) {
     const at::Tensor g = at::matmul(x_, wg.t()), u = at::matmul(x_, wu.t()), dh = at::matmul(dy, wd);
@@ -283,7 +286,7 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
     variable_list result(5);
     if (!grads[0].defined()) return result;
     const at::Tensor x_ = x.unpack(), wg = w_gate.unpack(), wu = w_up.unpack(), wd = w_down.unpack();
-    if (at::GradMode::is_enabled() || at::isTensorSubclassLike(grads[0])) return recorded(grads[0], x_, wg, wu, wd);
+    if (as_operations(grads[0])) return recorded(grads[0], x_, wg, wu, wd);
     if (with_residual) result[4] = grads[0];
     const at::Tensor h = hidden.unpack(), g = gate.unpack(), u = up.unpack(), l = low.unpack();
     const c10::cuda::CUDAGuard guard(x_.device());
