@@ -37,3 +37,9 @@ def test_whole_tiles_and_gradients(rows, n_in, n_mid, n_out):
 def test_fp32_tiles(rows, n_in, n_mid, n_out):
     for with_residual in (False, True):
         _check(rows, n_in, n_mid, n_out, torch.float32, "silu", with_residual, seed=43)
+
+
+@pytest.mark.parametrize("rows", [1, 16, 40, 300, 2100])
+@pytest.mark.parametrize("n_in,n_mid,n_out", [(65536, 8, 8), (8, 65536, 8), (8, 8, 65536), (65536, 24, 40)])
+def test_the_widest_and_the_narrowest(rows, n_in, n_mid, n_out):
+    _check(rows, n_in, n_mid, n_out, torch.bfloat16, "silu", rows % 2 == 0, seed=47)
