@@ -249,7 +249,10 @@ at::Tensor kernel_ready(const at::Tensor& t) {
 
 // Rows without gradients for which the kernels of gated_rows.cu are ahead of tiles of 128 rows.  us, weights not in the L2: 2,048 x
 // 5,632 x 2,048, one row 14.5 / 35, 16 rows 17 / 29, 32 rows 22 / 24; 768 x 2,048 x 768, 32 rows 9 / 14; 4,096 x 11,008 x 4,096, one row
-// 47 / 74, 32 rows 55 / 58; behind with 32 rows of 512 x 2,048 x 16,384 29 / 20, 4,096 x 14,336 x 4,096 82 / 70.
+// 47 / 74, 32 rows 55 / 58; behind with 32 rows of 512 x 2,048 x 16,384 29 / 20, 4,096 x 14,336 x 4,096 82 / 70.  16 rows: 64 x 128 x 64
+// 3.8 / 7.0, 768 x 2,048 x 768 7.5 / 14.6, 512 x 2,048 x 16,384 23 / 30, 1,024 x 4,096 x 16,384 37 / 40, 8,192 x 28,672 x 8,192 232 / 237,
+// alike at 4,096 x 14,336 x 4,096 (70 / 69) and 5,120 x 13,824 x 5,120 (90 / 88), behind at 8,192 x 8,192 x 8,192 (86 / 78) and with
+// middles of 64 outputs and more: 512 x 65,536 x 512 73 / 69, 128 x 65,536 x 128 65 / 47 (32 rows 82 / 47).
 bool few_rows(int64_t rows, int64_t in, int64_t mid, int64_t out) {
   return rows <= 16 || (rows <= 32 && out <= 4096 && in * mid <= int64_t(48) << 20);
 }

@@ -4,7 +4,9 @@
 //
 // bf16: five products of gated_gemm.cuh.  The gate's and the up projection's columns of a tile are summed side by side, so
 // the activation and their product are taken from fp32 sums before anything is rounded; dg and du leave the product that makes dh,
-// dx is one sum over both, and each weight's gradient is summed over rows that all SMs share.
+// dx is one sum over both, and each weight's gradient is summed over rows that all SMs share.  What goes from one product into the
+// next, h, dg and du, is rounded to bf16, the type the tensor cores take at twice the rate of any wider one: y is 1.9e-3 from 64 bits
+// in the 2-norm (its own rounding alone 1.7e-3), the gradients 2.3e-3.
 // fp32: the split products of linear_mma.cu with the gate in their finish, or, for reductions over several launches and few rows,
 // with the gate in kernels of its own.
 #include <atomic>

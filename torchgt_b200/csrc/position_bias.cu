@@ -11,8 +11,10 @@
 // group, head), so no two of them share a word or a bank, and what a hub's bucket costs is what any costs.  The sums
 // of a CTA's warps and then of the CTAs are added in a fixed order: no atomics, the same bits every time.  Both directions are bound by the
 // ids and the rows of bias; the forward keeps the buckets, 2 bytes an edge in the place of the 16 of two ids.
-// us, 18.2 M edges x 8 heads, 870,001 positions: forward 217 (910 MB; without positions 146: two random reads an edge keep the L1's
-// tags busy), backward 130 and 9 for the last sums (620 MB); 526,450 edges 8.5, 8.4 and 4.5.
+// The sums are fp32, a lane's own of up to some thousand terms: 1.2e-7 to 2.5e-7 from 64 bits in the 2-norm over all list lengths.
+// us, 18.2 M edges x 8 heads, 870,001 positions: forward 217 (910 MB; without positions 146: two random reads an edge are requests of
+// their own and keep the way to the L2 busy in 86 % of the cycles), backward 130 (issue slots 75 % busy, DRAM 56 %) and 9 for the
+// last sums (620 MB); 526,450 edges 8.5, 8.4 and 4.5.
 #include "tgt_common.cuh"
 
 namespace tgt {

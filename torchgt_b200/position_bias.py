@@ -79,7 +79,7 @@ def edge_position_bias(table: torch.Tensor, edge_index: torch.Tensor, positions:
     ``table`` is [num_buckets, H] fp32 (up to 512 buckets and 256 heads); ``positions`` [N] int64 or int32 holds the nodes'
     positions (None: a node's position is its id).  An edge with an id outside the positions gets NaN and has no part in the
     gradient: nothing waits for the GPU to raise.  The table's gradient is summed in a fixed order (the same bits every
-    time).  Raises if the tensors are not on one CUDA device: there is no CPU path."""
+    time; where it is itself differentiated it is torch's ``index_add``, whose order may change).  Raises if the tensors are not on one CUDA device: there is no CPU path."""
     if not isinstance(edge_index, torch.Tensor):
         raise TypeError("edge_index must be the [2, E] tensor of the edges: a SparseGraph has them in another order")
     tensors = [table, edge_index] + ([positions] if positions is not None else [])

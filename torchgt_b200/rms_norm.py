@@ -30,8 +30,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None)
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None,
                  want_sum: bool = True):
-    """``(rms_norm(x + residual), x + residual)`` in one kernel each way.  The norm is that of the sum before it is rounded to
-    the tensors' type.  The second is None when ``want_sum`` is false and nothing else needs it."""
+    """``(rms_norm(x + residual), x + residual)`` in one kernel each way.  The kernel's norm is that of the sum before it is
+    rounded to the tensors' type.  The second is None when ``want_sum`` is false and nothing else needs it."""
     if x.is_cuda and weight is not None and plain_call(x, residual, weight):
         out = _cabi.native().add_rms_norm(x, residual, weight, _eps(x, eps), want_sum)
         if out is not None:
