@@ -93,3 +93,13 @@ def test_positions_at_the_ends_of_64_bits_in_the_kernels(both_ways):
         assert torch.equal(got.cpu(), want)
         wrapped = torch.func.vmap(lambda t: edge_position_bias(t, ids.cuda(), where, bidirectional=both_ways))(table.cuda()[None])   # noqa: B023
         assert torch.equal(wrapped[0].cpu(), want)
+
+
+def test_a_trace_takes_other_lists_and_positions():
+    """Sizes of the traced call are not in the trace: more nodes, more edges, and an id outside the new ones."""
+    table = torch.randn(32, 4)
+    lists = lambda n, e, seed: (torch.randint(0, n, (2, e), generator=torch.Generator().manual_seed(seed)), torch.arange(n).flip(0) * 3)   # noqa: E731
+    traced = torch.jit.trace(_recorded, (table, *lists(50, 200, 1)), check_trace=False)
+    edges, positions = lists(80, 301, 2)
+    edges[0, 3], edges[1, 9] = 80, -1
+    assert _same(traced(table, edges, positions), _defined(table, edges, positions))
